@@ -66,6 +66,12 @@ typedef int sa_status;
 #define SA_DEV_NONFINITE 0x8u    /* a block score was NaN or infinite        */
 #define SA_DEV_TIMEOUT 0x10u     /* a bounded barrier wait gave up           */
 #define SA_DEV_TABLE_FULL 0x20u  /* seal beyond the block-table capacity     */
+#define SA_DEV_SLOTS_FULL 0x40u  /* more new tokens than the slot map holds  */
+
+/* Element types of the calls that take more than one. */
+#define SA_TYPE_F32 0
+#define SA_TYPE_F16 1
+#define SA_TYPE_BF16 2
 
 SA_API const char* sa_status_string(sa_status status);
 /* Message of the last failing call on this host thread ("" if none). */
@@ -160,6 +166,127 @@ SA_API sa_status sa_build_representatives(
 SA_API sa_status sa_pack_kv_fp16(uint16_t* packed, const float* key,
                                  const float* value, size_t token,
                                  size_t elements, void* stream);
+
+/* ------------------------------------------------- 4-bit paged cache (kv4)
+ *
+ * A paged K/V cache held in 4 bits, its block tables planned on the device.
+ * None of these calls has a counterpart in the reference, whose caches are
+ * FP16; block size, block tables, the free list and the selected-block ids are
+ * those of the paged decode context below. All pointers are device memory of
+ * the current device, and every call is asynchronous on `stream`, allocates
+ * nothing, reads lengths and tables on the device only and can be captured in
+ * a CUDA graph. `status` is a device word that kernels OR SA_DEV_* bits into,
+ * or null; the caller clears it.
+ *
+ * Pool: uint8 [pool_blocks][kv_heads][36 * head_dim], 16-byte aligned, one
+ * entry per (32-token block, KV head): key codes, value codes, key scales,
+ * value scales (16, 16, 2 and 2 * head_dim bytes). Rows are quantised in
+ * groups of 64 elements, 4.5 bits an element in all:
+ *
+ *   minimum m = largest FP16 value <= the group's smallest element,
+ *   step    s = smallest FP16 value >= (largest element - m) / 15,
+ *   code    c = (x - m) / s rounded to nearest, ties to even (0 if s = 0),
+ *   the value held is s * c + m: within s / 2 of x.
+ *
+ * Finite elements are first clamped to +-65504; a NaN or infinite element
+ * makes its whole group NaN. head_dim is 64, 128 or 256. */
+SA_API size_t sa_kv4_entry_bytes(size_t head_dim);
+
+/* Bring a batch's block tables, lengths and free list from one step to the
+ * next and map every new token to its slot (32 * physical block + row).
+ *   add         [requests]: tokens appended to (> 0) or taken back from the end
+ *               of (< 0, at most all of them) each request in this step.
+ *   seq_lens    [requests], in place: tokens held.
+ *   block_table [requests][table_blocks], in place: logical -> physical block;
+ *               entries beyond a request's blocks keep their old contents.
+ *   free_list   [pool_blocks], free_top [1], in place: stack of free blocks.
+ *   slots_out   [max_tokens]: slots of the new tokens, request by request,
+ *               then -1.
+ *   positions_out [max_tokens] (nullable): their positions, then 0.
+ *   cu_tokens_out [requests + 1] (nullable): first row of each request's new
+ *               tokens, and their number.
+ * Blocks are taken in request order from the top of the list as it stood, and
+ * those given back are pushed after that in reverse order, so that a step
+ * followed by its inverse restores the list. A request whose growth does not
+ * fit is refused: its length, blocks and table row stay, its tokens get slot
+ * -1, and a status bit is set: SA_DEV_TABLE_FULL (the table's row is too
+ * short), SA_DEV_SLOTS_FULL (its tokens end beyond max_tokens),
+ * SA_DEV_POOL_EMPTY (the blocks that it and the requests before it need exceed
+ * the free ones). SA_DEV_BAD_BLOCK: a length, table entry or list entry was
+ * outside its range. requests <= 8192. */
+SA_API sa_status sa_plan_blocks(const int32_t* add, size_t requests,
+                                int32_t* seq_lens, int32_t* block_table,
+                                size_t table_blocks, int32_t* free_list,
+                                size_t pool_blocks, int32_t* free_top,
+                                size_t max_tokens, int32_t* slots_out,
+                                int32_t* positions_out, int32_t* cu_tokens_out,
+                                uint32_t* status, void* stream);
+
+/* Quantise `tokens` rows of keys and values into the slots of a pool.
+ * key, value: [tokens][kv_heads][head_dim] of `type` (SA_TYPE_*), element
+ * (t, h, d) at key[t * key_token_stride + h * key_head_stride + d] (strides in
+ * elements). Rows with a negative slot are skipped; a slot beyond the pool is
+ * skipped and sets SA_DEV_BAD_BLOCK. Slots of one call must differ: of rows
+ * that share a slot, pieces of each may be kept. */
+SA_API sa_status sa_pack_kv4(void* pool, size_t pool_blocks, const void* key,
+                             const void* value, int type,
+                             int64_t key_token_stride, int64_t key_head_stride,
+                             int64_t value_token_stride,
+                             int64_t value_head_stride, const int32_t* slots,
+                             size_t tokens, size_t kv_heads, size_t head_dim,
+                             uint32_t* status, void* stream);
+
+/* The rows held in `tokens` slots, as `type`: the values (FP32, rounded once)
+ * in key_out and value_out [tokens][kv_heads][head_dim], 16-byte aligned. Rows
+ * with a negative slot are zeros; a slot beyond the pool gives zeros and sets
+ * SA_DEV_BAD_BLOCK. */
+SA_API sa_status sa_unpack_kv4(const void* pool, size_t pool_blocks,
+                               const int32_t* slots, size_t tokens,
+                               size_t kv_heads, size_t head_dim, void* key_out,
+                               void* value_out, int type, uint32_t* status,
+                               void* stream);
+
+/* GQA attention of the newest tokens of a batch over a 4-bit pool, dense or
+ * over selected blocks.
+ *   query [requests][new_tokens][query_heads][head_dim] of query_type, element
+ *         (b, i, h, d) at query[b * stride_request + i * stride_token +
+ *         h * stride_head + d] (strides in elements).
+ *   block_table [requests][table_blocks]; seq_lens [requests]: tokens held, the
+ *         new ones included. Query i of request b stands at position
+ *         seq_lens[b] - new_tokens + i and sees positions up to its own; one
+ *         that sees none gives zeros (and -inf in lse_out).
+ *   selected (nullable: every block) [requests][select_groups][budget]: logical
+ *         ids, ascending and unique, selected_count [requests][select_groups]
+ *         of them in use; KV heads share a list in groups of kv_heads /
+ *         select_groups, as in the decode context. The block of the newest token is
+ *         always attended and is not listed. Needs new_tokens = 1. An id that
+ *         is out of range or not above the one before it is skipped and sets
+ *         SA_DEV_BAD_BLOCK, as does a table entry outside the pool.
+ *   out   [requests][new_tokens][query_heads][head_dim] of out_type: query_type
+ *         if that has 16 bits, any if it is SA_TYPE_F32.
+ *   lse_out (nullable) [requests][new_tokens][query_heads] FP32: the natural
+ *         logarithm of the sum of exponentials, for merging with attention over
+ *         another cache.
+ * A negative length, or one above 32 * table_blocks, counts as zero and sets
+ * SA_DEV_BAD_BLOCK. Logits, softmax and sums are FP32. query_heads is a
+ * multiple of kv_heads; requests * select_groups (requests, when dense) <= 8192.
+ * workspace: device scratch of sa_attention_kv4_workspace_size() bytes,
+ * 16-byte aligned; it needs no initialisation, and calls that may overlap in
+ * time need one each. */
+SA_API size_t sa_attention_kv4_workspace_size(size_t requests,
+                                              size_t new_tokens,
+                                              size_t query_heads,
+                                              size_t kv_heads,
+                                              size_t head_dim);
+SA_API sa_status sa_attention_kv4(
+    const void* query, int query_type, int64_t stride_request,
+    int64_t stride_token, int64_t stride_head, const void* pool,
+    size_t pool_blocks, const int32_t* block_table, size_t table_blocks,
+    const int32_t* seq_lens, const int32_t* selected,
+    const int32_t* selected_count, size_t select_groups, size_t budget,
+    size_t requests, size_t new_tokens, size_t query_heads, size_t kv_heads,
+    size_t head_dim, float scale, void* out, int out_type, float* lse_out,
+    void* workspace, size_t workspace_bytes, uint32_t* status, void* stream);
 
 /* ---------------------------------------------------------- backend handle */
 

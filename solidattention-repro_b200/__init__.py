@@ -12,6 +12,10 @@ Names and argument meanings follow the reference (ZjuXxxc/solidattention-repro):
 * :class:`DecodeContext`             -- the P1.3 KV lifecycle,
   cpp/src/kv_lifecycle_main.cpp:25-113 and cpp/src/online_seal_main.cpp:34-47
 
+The 4-bit paged cache has no counterpart there (:mod:`.kv4`):
+:func:`plan_blocks`, :func:`kv4_pool`, :func:`pack_kv4`, :func:`unpack_kv4`,
+:func:`attention_kv4`.
+
 Invalid dimensions raise :class:`SparseKVError` with status
 ``SA_ERR_INVALID_ARG`` where the reference throws ``std::runtime_error``.
 """
@@ -25,13 +29,15 @@ import numpy as np
 import torch
 
 from ._lib import (SA_ATTN_CONSUME, SA_ATTN_COPY_OUTPUT, SA_DEV_BAD_BLOCK, SA_DEV_NONFINITE,
-                   SA_DEV_POOL_EMPTY, SA_DEV_TABLE_FULL, SA_DEV_TAIL_FULL, SA_DEV_TIMEOUT,
+                   SA_DEV_POOL_EMPTY, SA_DEV_SLOTS_FULL, SA_DEV_TABLE_FULL, SA_DEV_TAIL_FULL,
+                   SA_DEV_TIMEOUT,
                    SA_ERR_CAPACITY, SA_ERR_DEVICE, SA_ERR_INVALID_ARG, SA_ERR_TIMEOUT,
                    SA_ERR_UNSUPPORTED, CtxConfig, CtxPtrs, SparseKVError, Timings, check, load)
 
 __all__ = [
     "attention", "select_shared_blocks", "build_local_causal_representatives", "pack_kv_fp16",
     "Backend", "DecodeContext", "SparseKVError", "load", "version",
+    "plan_blocks", "kv4_pool", "pack_kv4", "unpack_kv4", "attention_kv4",
 ]
 
 BLOCK_TOKENS = 32
@@ -539,3 +545,6 @@ class DecodeContext:
             self.close()
         except Exception:
             pass
+
+
+from .kv4 import attention_kv4, kv4_pool, pack_kv4, plan_blocks, unpack_kv4  # noqa: E402

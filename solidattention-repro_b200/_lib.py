@@ -26,6 +26,11 @@ SA_DEV_POOL_EMPTY = 0x4
 SA_DEV_NONFINITE = 0x8
 SA_DEV_TIMEOUT = 0x10
 SA_DEV_TABLE_FULL = 0x20
+SA_DEV_SLOTS_FULL = 0x40
+
+SA_TYPE_F32 = 0
+SA_TYPE_F16 = 1
+SA_TYPE_BF16 = 2
 
 SA_ATTN_COPY_OUTPUT = 0x1
 SA_ATTN_CONSUME = 0x2
@@ -79,6 +84,16 @@ PROTOTYPES = {
     "sa_build_representatives": (C.c_int, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _vp,
                                            _vp, _vp]),
     "sa_pack_kv_fp16": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _vp]),
+    "sa_kv4_entry_bytes": (_sz, [_sz]),
+    "sa_plan_blocks": (C.c_int, [_vp, _sz, _vp, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp,
+                                 _vp]),
+    "sa_pack_kv4": (C.c_int, [_vp, _sz, _vp, _vp, C.c_int, _i64, _i64, _i64, _i64, _vp, _sz, _sz,
+                              _sz, _vp, _vp]),
+    "sa_unpack_kv4": (C.c_int, [_vp, _sz, _vp, _sz, _sz, _sz, _vp, _vp, C.c_int, _vp, _vp]),
+    "sa_attention_kv4_workspace_size": (_sz, [_sz, _sz, _sz, _sz, _sz]),
+    "sa_attention_kv4": (C.c_int, [_vp, C.c_int, _i64, _i64, _i64, _vp, _sz, _vp, _sz, _vp, _vp,
+                                   _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, C.c_float, _vp,
+                                   C.c_int, _vp, _vp, _sz, _vp, _vp]),
     "sa_backend_create": (C.c_int, [C.c_int, C.POINTER(_vp)]),
     "sa_backend_destroy": (C.c_int, [_vp]),
     "sa_backend_name": (C.c_char_p, [_vp]),
