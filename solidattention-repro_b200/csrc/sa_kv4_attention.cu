@@ -4,15 +4,51 @@
 //   x_t = scale * sum_d q_d (s_t,g c_t,d + m_t,g)      softmax over the tokens seen
 //   o_d = sum_t p_t (s'_t,g c'_t,d + m'_t,g) / sum_t p_t
 //
-// One CTA per (request, new token, query head): each warp walks its share of
-// the row's blocks, a lane scoring one token and owning D / 32 output elements,
-// with a running maximum and sum; the warps are merged at the end.
+// The codes are never dequantised. A nibble in the low bits of a 16-bit lane is
+// an FP16 subnormal, c * 2^-24 (c * 2^-20 for the next nibble, whose factor 16
+// goes into the query for keys and into the output row for values), so one AND
+// turns eight codes into a matrix operand register pair, and the tensor cores
+// multiply codes exactly:
+//
+//   x_t = F sum_g s_t,g (sum_d q'_d c_t,d) + sum_g m_t,g Q_g,   Q_g = sum_d q_d
+//   o_d = sum_t (p_t s'_t,g) c'_t,d + sum_t p_t m'_t,g
+//
+// with q' = q scaled by a power of two per row to [2^14, 2^15), the key scales
+// applied to the FP32 products, and the value steps folded into the FP16
+// weights (one extra matrix row a group gives the second sum). Tokens are the
+// matrix rows of the first product and query rows its columns, so that up to 8
+// query rows (heads of a KV head times new tokens) cost one m16n8k16 column
+// tile; the weights become the second product's operand by an 8x8 transpose of
+// registers (movmatrix).
+//
+// Rounding. FP32 queries are split into two FP16 parts. Weights are rounded to
+// FP16 once where the output is BF16 (2^-11 against its 2^-8) and split into
+// two parts otherwise. There the value codes are also centred, c - 8 with
+// minimum + 8 step (in two FP16 parts): over a long context the output is a
+// small difference of large sums otherwise, and the matrix unit's truncating
+// sums lost 1e-4 of it at 4,128 tokens (9e-7 for plain FP32). FP32 queries
+// centre the key codes too, and add the products of their small parts apart.
+// Logits, maxima, sums and partial results are FP32. Value
+// steps are scaled by a power of two that follows their running maximum E, so
+// that weight * step stays inside FP16: steps 2^-24 below the largest one seen
+// by a warp vanish next to it.
+//
+// Work split. All (list, KV head, row tile) units' entries form one flat list;
+// every warp takes an equal contiguous range of it, whatever the lengths, and
+// streams its entries through a ring of its own. A unit that a warp covers
+// alone is written at once; parts of units go to the workspace as (max, sum,
+// weighted values) and merge_kernel joins them in list order.
+#include <algorithm>
+
 #include "sa_kv4.cuh"
 
 namespace sa {
 namespace {
 
 constexpr int kMaxLists = 8192;
+constexpr int kWarps = 8;        // of a CTA
+constexpr float kHeadroom = 4.0f;  // log2 by which a weight may exceed its row's running maximum
+constexpr float kWeightLog2 = 11.0f;  // weights are held as 2^11 p: at most 2^15 in FP16
 
 struct Kv4AttnParams {
   const void* query;
@@ -27,9 +63,19 @@ struct Kv4AttnParams {
   float* lse;
   uint32_t* status;
   int pool_blocks, table_blocks, lists_per_request, budget;
-  int requests, new_tokens, query_heads, kv_heads, head_dim;
-  float scale;
+  int requests, new_tokens, query_heads, kv_heads;
+  int group;           // query heads per KV head
+  int rows;            // query rows of a KV head: group * new_tokens
+  int row_tiles;       // tiles of 8 * NT rows
+  int units_per_list;  // KV heads of a list * row_tiles
+  float scale_log2;    // softmax scale * log2(e)
+  int ctas;            // of the attention grid
+  int* starts;         // workspace: [lists + 1] entries of the lists before each
+  float* part_ml;      // workspace: [warps][2][rows of a tile][max, sum]
+  float* part_o;       // workspace: [warps][2][rows of a tile][head_dim]
 };
+
+// ---- elements of the calls' types ------------------------------------------------
 
 __device__ __forceinline__ float load_as_float(const void* base, int64_t i, int type) {
   if (type == SA_TYPE_F32) return static_cast<const float*>(base)[i];
@@ -37,126 +83,788 @@ __device__ __forceinline__ float load_as_float(const void* base, int64_t i, int 
   return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
 }
 
-__device__ __forceinline__ void store_from_float(void* base, int64_t i, int type, float x) {
-  if (type == SA_TYPE_F32)
-    static_cast<float*>(base)[i] = x;
-  else if (type == SA_TYPE_F16)
-    static_cast<__half*>(base)[i] = __float2half_rn(x);
-  else
-    static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A request's length, 0 (and a status bit) when it is out of range.
-__device__ __forceinline__ int checked_length(int length, int table_blocks, uint32_t* status) {
-  if (length >= 0 && length <= static_cast<int64_t>(table_blocks) * kBlockTokens) return length;
-  raise_status(status, SA_DEV_BAD_BLOCK);
-  return 0;
+__device__ __forceinline__ uint32_t pack_bf162(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-constexpr int kWarps = 4;
+// Eight consecutive elements from element `i` on (a multiple of 8).
+__device__ __forceinline__ void store8(void* base, int64_t i, int type, const float (&x)[8]) {
+  if (type == SA_TYPE_F32) {
+    float4* at = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
+    at[0] = make_float4(x[0], x[1], x[2], x[3]);
+    at[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else if (type == SA_TYPE_F16) {
+    *reinterpret_cast<uint4*>(static_cast<__half*>(base) + i) =
+        make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]),
+                   pack_half2(x[6], x[7]));
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + i) =
+        make_uint4(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]), pack_bf162(x[4], x[5]),
+                   pack_bf162(x[6], x[7]));
+  }
+}
 
-__global__ void __launch_bounds__(kWarps * 32) attention_simple(const Kv4AttnParams p) {
-  __shared__ float q[256];
-  __shared__ float part[kWarps][2 + 256];
-  const int d = p.head_dim, per_lane = d / 32, groups = d / kKv4Group;
-  const int row = blockIdx.x;
-  const int head = row % p.query_heads, i = row / p.query_heads % p.new_tokens;
-  const int b = row / p.query_heads / p.new_tokens;
-  const int kv_head = head / (p.query_heads / p.kv_heads);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < d; e += blockDim.x)
-    q[e] = load_as_float(p.query, b * p.stride_request + i * p.stride_token +
-                                      head * p.stride_head + e, p.query_type);
+// ---- matrix fragments -------------------------------------------------------------
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8x8 matrix of 16-bit elements held one row per four lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                            *reinterpret_cast<const __half2*>(&c));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
+  const __half2 r = __hadd2_rn(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  return hadd2(a, b ^ 0x80008000u);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t a) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&a));
+}
+
+constexpr uint32_t kNibble0 = 0x000f000fu;  // c * 2^-24 in both halves
+constexpr uint32_t kNibble1 = 0x00f000f0u;  // c * 2^-20
+
+// Codes as an operand register: c * 2^-24, or centred c - 8 (1024 + c,
+// then minus 1032); the odd ones are 16 times that.
+template <bool CENTRED>
+__device__ __forceinline__ uint32_t even_codes(uint32_t word) {
+  return CENTRED ? hadd2((word & kNibble0) | 0x64006400u, 0xe408e408u) : word & kNibble0;
+}
+template <bool CENTRED>
+__device__ __forceinline__ uint32_t odd_codes(uint32_t word) {
+  return CENTRED ? hadd2((word & kNibble1) | 0x64006400u, 0xe480e480u) : word & kNibble1;
+}
+
+// ---- lists and units ----------------------------------------------------------------
+
+// A request's length, 0 when it is out of range.
+__device__ __forceinline__ int checked_length(int length, int table_blocks) {
+  return length >= 0 && length <= static_cast<int64_t>(table_blocks) * kBlockTokens ? length : 0;
+}
+
+// Entries of a list: its request's blocks, or the selected ones and the newest.
+__device__ __forceinline__ int list_entries(const Kv4AttnParams& p, int list, bool* bad) {
+  const int raw = p.seq_lens[list / p.lists_per_request];
+  const int length = checked_length(raw, p.table_blocks);
+  *bad = length != raw;
+  if (length == 0) return 0;
+  if (!p.selected) return (length + kBlockTokens - 1) / kBlockTokens;
+  return min(max(p.selected_count[list], 0), p.budget) + 1;
+}
+
+// The last list whose first entry is not behind `at`.
+__device__ __forceinline__ int list_of(const int* starts, int lists, int at) {
+  int low = 0, high = lists;
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (starts[mid] <= at)
+      low = mid;
+    else
+      high = mid;
+  }
+  return low;
+}
+
+// Flat entries a warp takes.
+__device__ __forceinline__ int64_t quota_of(int64_t entries, int64_t warps) {
+  return max((entries + warps - 1) / warps, static_cast<int64_t>(1));
+}
+
+// ---- attention -------------------------------------------------------------------------
+
+template <int NG>
+struct Ring {
+  static constexpr int kEntry = 36 * 64 * NG;
+  static constexpr int kStages = NG == 4 ? 2 : 3;
+  static constexpr int kBytes = kWarps * kStages * kEntry;
+};
+
+template <int NG, int NT, int MODE>
+constexpr int min_ctas() {
+  return NG <= 2 && NT == 1 ? 2 : 1;
+}
+
+// MODE 0: 16-bit queries, BF16 output. 1: 16-bit queries, FP16 output (weights
+// in two parts). 2: FP32 queries (queries and weights in two parts).
+template <int NG, int NT, int MODE>
+__global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
+    attention_kernel(const Kv4AttnParams p) {
+  constexpr int kDim = 64 * NG, kEntry = Ring<NG>::kEntry, kStages = Ring<NG>::kStages;
+  constexpr int kTile = 8 * NT;               // query rows of a unit
+  constexpr int kParts = MODE == 2 ? 2 : 1;   // FP16 parts of a query
+  constexpr int kWeights = MODE == 0 ? 1 : 2;  // FP16 parts of a weight
+  constexpr bool kCentred = kWeights == 2;    // value codes as c - 8
+  constexpr bool kCentredKeys = kParts == 2;  // key codes too
+  constexpr int kPieces = kEntry / 16;        // 16-byte pieces of an entry
+  extern __shared__ __align__(128) uint8_t kv4_smem[];
+  __shared__ int scan_scratch[33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  uint8_t* ring = kv4_smem + warp * kStages * kEntry;
+  int* starts = reinterpret_cast<int*>(kv4_smem + Ring<NG>::kBytes);
+  const int lists = p.requests * p.lists_per_request;
+
+  pdl_launch_dependents();
+  // Entries before each list.
+  int base = 0;
+  for (int first = 0; first < lists; first += blockDim.x) {
+    const int list = first + threadIdx.x;
+    bool bad = false;
+    const int n = list < lists ? list_entries(p, list, &bad) : 0;
+    if (bad && blockIdx.x == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
+    int total;
+    const int before = base + block_exclusive_scan(n, scan_scratch, &total);
+    if (list < lists) starts[list] = before;
+    base += total;
+  }
+  if (threadIdx.x == 0) starts[lists] = base;
   __syncthreads();
-  const int length = checked_length(p.seq_lens[b], p.table_blocks, p.status);
-  const int seen = length - p.new_tokens + i + 1;  // tokens this row sees
-  const int blocks = (length + kBlockTokens - 1) / kBlockTokens;
-  const int list = b * p.lists_per_request + kv_head / (p.kv_heads / p.lists_per_request);
-  const int32_t* ids = p.selected ? p.selected + static_cast<int64_t>(list) * p.budget : nullptr;
-  int entries = blocks;
-  if (ids && blocks > 0) entries = min(max(p.selected_count[list], 0), p.budget) + 1;
-  float top = -INFINITY, sum = 0.0f, o[8] = {};
-  for (int e = warp; e < entries; e += kWarps) {
-    int logical = e;
-    if (ids) {
-      logical = blocks - 1;
-      if (e < entries - 1) {
-        logical = ids[e];
-        if (logical < 0 || logical >= blocks - 1 || (e > 0 && logical <= ids[e - 1])) {
-          raise_status(p.status, SA_DEV_BAD_BLOCK);
-          continue;
-        }
-      }
-    }
-    const int block = p.table[static_cast<int64_t>(b) * p.table_blocks + logical];
-    if (block < 0 || block >= p.pool_blocks) {
-      raise_status(p.status, SA_DEV_BAD_BLOCK);
-      continue;
-    }
-    const uint8_t* entry = p.pool + (static_cast<int64_t>(block) * p.kv_heads + kv_head) *
-                                        kv4_entry_bytes(d);
-    const bool sees = logical * kBlockTokens + lane < seen;
-    float x = -INFINITY;
-    if (sees) {
-      x = 0.0f;
-      for (int g = 0; g < groups; ++g) {
-        float dot = 0.0f, all = 0.0f;
-        for (int t = 0; t < 4; ++t) {
-          const uint2 w = *reinterpret_cast<const uint2*>(entry + kv4_key_at(d, lane, g, t));
-          for (int j = 0; j < 16; ++j) {
-            const float qj = q[g * kKv4Group + 16 * t + j];
-            dot += qj * static_cast<float>(((j < 8 ? w.x : w.y) >> (4 * (j & 7))) & 15u);
-            all += qj;
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= lists; i += blockDim.x) p.starts[i] = starts[i];
+
+  const int64_t entries = static_cast<int64_t>(base) * p.units_per_list;
+  const int64_t quota = quota_of(entries, static_cast<int64_t>(p.ctas) * kWarps);
+  // Neighbouring ranges go to different SMs: few entries still use them all.
+  const int64_t range = static_cast<int64_t>(warp) * p.ctas + blockIdx.x;
+  int64_t at = range * quota;
+  const int64_t end = min(at + quota, entries);
+
+  while (at < end) {
+    // The unit of flat entry `at`, and the part of it in this warp's range.
+    const int list = list_of(starts, lists, static_cast<int>(at / p.units_per_list));
+    const int n = starts[list + 1] - starts[list];
+    const int64_t in_list = at - static_cast<int64_t>(starts[list]) * p.units_per_list;
+    const int unit = static_cast<int>(in_list / n), first = static_cast<int>(in_list % n);
+    const int count = static_cast<int>(min(static_cast<int64_t>(n - first), end - at));
+    const int b = list / p.lists_per_request;
+    const int kv_head = list % p.lists_per_request * (p.kv_heads / p.lists_per_request) +
+                        unit / p.row_tiles;
+    const int row0 = unit % p.row_tiles * kTile;
+    const int length = checked_length(p.seq_lens[b], p.table_blocks);
+    const int newest = (length - 1) / kBlockTokens;
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_blocks;
+    const int32_t* ids =
+        p.selected ? p.selected + static_cast<int64_t>(list) * p.budget : nullptr;
+    const uint8_t* head_pool = p.pool + static_cast<int64_t>(kv_head) * kEntry;
+    const int64_t block_stride = static_cast<int64_t>(p.kv_heads) * kEntry;
+
+    // Physical blocks of 32 entries from `from` on, one per lane; -1 where
+    // there is none to read.
+    auto blocks_from = [&](int from) {
+      const int e = from + lane;
+      int block = -1;
+      if (e < first + count) {
+        int logical = e;
+        bool good = true;
+        if (ids) {
+          logical = newest;
+          if (e < n - 1) {
+            logical = ids[e];
+            good = logical >= 0 && logical < newest && (e == 0 || logical > ids[e - 1]);
           }
         }
-        const __half2 sm =
-            *reinterpret_cast<const __half2*>(entry + kv4_key_scale_at(d, lane, g));
-        x += __low2float(sm) * dot + __high2float(sm) * all;
+        if (good) block = table[logical];
+        if (block < 0 || block >= p.pool_blocks) {
+          block = -1;
+          raise_status(p.status, SA_DEV_BAD_BLOCK);
+        }
       }
-      x *= p.scale;
-    }
-    float new_top = fmaxf(top, x);
-    for (int s = 16; s > 0; s >>= 1)
-      new_top = fmaxf(new_top, __shfl_xor_sync(0xffffffffu, new_top, s));
-    if (new_top == -INFINITY) continue;
-    const float keep = expf(top - new_top), pr = sees ? expf(x - new_top) : 0.0f;
-    top = new_top;
-    float block_sum = pr;
-    for (int s = 16; s > 0; s >>= 1) block_sum += __shfl_xor_sync(0xffffffffu, block_sum, s);
-    sum = sum * keep + block_sum;
-    for (int j = 0; j < per_lane; ++j) o[j] *= keep;
-    for (int r = 0; r < kBlockTokens; ++r) {
-      if (logical * kBlockTokens + r >= seen) break;
-      const float pt = __shfl_sync(0xffffffffu, pr, r);
-      for (int j = 0; j < per_lane; ++j) {
-        const int el = lane * per_lane + j, g = el / kKv4Group, in = el % kKv4Group;
-        const uint32_t byte =
-            entry[kv4_value_at(d, r, g, in / 8, in % 8 / 4, in % 4 / 2)];
-        const __half* at = reinterpret_cast<const __half*>(entry + kv4_value_scale_at(d, r, g));
-        o[j] += pt * (__half2float(at[0]) * static_cast<float>((byte >> (4 * (in & 1))) & 15u) +
-                      __half2float(at[d / 2]));
+      return block;
+    };
+    int blocks = blocks_from(first);
+    uint32_t unread = 0;  // bit s: stage s holds no entry
+    auto fetch = [&](int i, int stage) {  // entry first + i into a stage
+      if (i < count) {
+        if (i > 0 && (i & 31) == 0) blocks = blocks_from(first + i);
+        const int block = __shfl_sync(0xffffffffu, blocks, i & 31);
+        unread &= ~(1u << stage);
+        if (block < 0) {
+          unread |= 1u << stage;
+        } else {
+          const uint8_t* from = head_pool + block * block_stride;
+          uint8_t* to = ring + stage * kEntry;
+#pragma unroll
+          for (int k = 0; k < (kPieces + 31) / 32; ++k) {
+            const int piece = k * 32 + lane;
+            if (kPieces % 32 == 0 || piece < kPieces) cp_async16(to + piece * 16, from + piece * 16);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) fetch(s, s);
+
+    // Query fragments: lane (g, t) holds elements 64 gr + 16 t .. + 15 of row g.
+    uint32_t q[NT][kParts][NG][8];
+    float row_factor[NT][2];   // F of columns 2t, 2t + 1
+    float row_sum[NT][NG][2];  // Q_g of columns 2t, 2t + 1
+    int limit[NT][2];          // tokens that columns 2t, 2t + 1 see
+    bool row_live[NT][2];
+    int least = length;  // tokens that every row sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + nt * 8 + g;
+      const bool live = row < p.rows;
+      const int i = live ? row / p.group : 0, h = live ? row % p.group : 0;
+      const int64_t from = b * p.stride_request + i * p.stride_token +
+                           (static_cast<int64_t>(kv_head) * p.group + h) * p.stride_head + 16 * t;
+      float x[NG][16], sums[NG];
+      float top = 0.0f;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        sums[gr] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          x[gr][e] = live ? load_as_float(p.query, from + 64 * gr + e, p.query_type) : 0.0f;
+          top = fmaxf(top, fabsf(x[gr][e]));
+          sums[gr] += x[gr][e];
+        }
+        sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], 1);
+        sums[gr] += __shfl_xor_sync(0xffffffffu, sums[gr], 2);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(14 - floor(log2 top)), kept inside FP32 for the smallest rows
+      const int exponent = max((__float_as_int(top) >> 23) - 127, -100);
+      const float up = __int_as_float((14 - exponent + 127) << 23);
+      const float down = __int_as_float((exponent - 14 + 127) << 23);
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int e = 8 * w + 2 * s;
+            const float even0 = x[gr][e] * up, even1 = x[gr][e + 4] * up;
+            const float odd0 = x[gr][e + 1] * up * 0.0625f, odd1 = x[gr][e + 5] * up * 0.0625f;
+            const int k = (w * 2 + s) * 2;
+            q[nt][0][gr][k] = pack_half2(even0, even1);
+            q[nt][0][gr][k + 1] = pack_half2(odd0, odd1);
+            if constexpr (kParts == 2) {
+              const float2 he = half2_floats(q[nt][0][gr][k]), ho = half2_floats(q[nt][0][gr][k + 1]);
+              q[nt][1][gr][k] = pack_half2(even0 - he.x, even1 - he.y);
+              q[nt][1][gr][k + 1] = pack_half2(odd0 - ho.x, odd1 - ho.y);
+            }
+          }
+      const float factor = p.scale_log2 * down * (kCentredKeys ? 1.0f : 16777216.0f);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int source = (2 * t + c) * 4;
+        row_factor[nt][c] = __shfl_sync(0xffffffffu, factor, source);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          row_sum[nt][gr][c] = p.scale_log2 * __shfl_sync(0xffffffffu, sums[gr], source);
+        const int r = row0 + nt * 8 + 2 * t + c;
+        row_live[nt][c] = r < p.rows;
+        limit[nt][c] = length - p.new_tokens + 1 + (row_live[nt][c] ? r / p.group : 0);
       }
     }
+    least = length - p.new_tokens + 1 + row0 / p.group;  // the tile's first row sees least
+
+    float o[NT][NG][2][2][4];  // codes' sums of element 64 gr + 8 g + 4 w + 2 s (+ 1, times 16)
+    float low[NT][2];          // minima's sums: lane group g holds value group g's
+    float top[NT][2], sum[NT][2];
+    int step_log2 = -64;  // E: value steps are held as s * 2^-E
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        top[nt][c] = -3.0e38f;
+        sum[nt][c] = 0.0f;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) low[nt][c] = 0.0f;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[nt][gr][m >> 1][m & 1][c] = 0.0f;
+    }
+
+    int stage = 0;
+    for (int i = 0; i < count; ++i) {
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      if (!(unread >> stage & 1)) {
+        const uint8_t* entry = ring + stage * kEntry;
+        const bool last = first + i == n - 1;
+        // first token of the block, in a dense list or the newest block
+        const int token0 = (ids ? newest : first + i) * kBlockTokens;
+        const int held = last ? length - newest * kBlockTokens : kBlockTokens;
+        const bool masked = (ids ? last : true) && token0 + kBlockTokens > least;
+
+        // ---- logits
+        float x[NT][2][4];
+        uint4 scales[NG];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          scales[gr] = *reinterpret_cast<const uint4*>(entry + kv4_key_scales(kDim) + gr * 128 + g * 16);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t word[2][2 * NG];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint8_t* from = entry + (16 * j + 8 * h + g) * (kDim / 2) + 8 * NG * t;
+            if constexpr (NG == 1) {
+              const uint2 w = *reinterpret_cast<const uint2*>(from);
+              word[h][0] = w.x;
+              word[h][1] = w.y;
+            } else {
+#pragma unroll
+              for (int k = 0; k < NG / 2; ++k) {
+                const uint4 w = *reinterpret_cast<const uint4*>(from + 16 * k);
+                word[h][4 * k] = w.x;
+                word[h][4 * k + 1] = w.y;
+                word[h][4 * k + 2] = w.z;
+                word[h][4 * k + 3] = w.w;
+              }
+            }
+          }
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr) {
+            float acc[NT][kParts][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[nt][part][c] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+              for (int s = 0; s < 2; ++s) {
+                const uint32_t r0 = word[0][2 * gr + w] >> (8 * s), r1 = word[1][2 * gr + w] >> (8 * s);
+                const uint32_t a0 = even_codes<kCentredKeys>(r0), a1 = even_codes<kCentredKeys>(r1),
+                               a2 = odd_codes<kCentredKeys>(r0), a3 = odd_codes<kCentredKeys>(r1);
+                const int k = (w * 2 + s) * 2;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int part = 0; part < kParts; ++part)
+                    mma16816(acc[nt][part], a0, a1, a2, a3, q[nt][part][gr][k], q[nt][part][gr][k + 1]);
+              }
+            const uint32_t sm0 = j == 0 ? scales[gr].x : scales[gr].z;
+            const uint32_t sm1 = j == 0 ? scales[gr].y : scales[gr].w;
+            float2 f0 = half2_floats(sm0), f1 = half2_floats(sm1);
+            if constexpr (kCentredKeys) {
+              f0.y = fmaf(8.0f, f0.x, f0.y);
+              f1.y = fmaf(8.0f, f1.x, f1.y);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float step = c < 2 ? f0.x : f1.x, minimum = c < 2 ? f0.y : f1.y;
+                const float lowest = minimum * row_sum[nt][gr][c & 1];
+                const float dot =
+                    kParts == 2 ? acc[nt][0][c] + acc[nt][kParts - 1][c] : acc[nt][0][c];
+                const float term = fmaf(step * dot, row_factor[nt][c & 1], lowest);
+                x[nt][j][c] = gr == 0 ? term : x[nt][j][c] + term;
+              }
+          }
+        }
+        if (masked) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (token0 + 16 * j + 8 * (c >> 1) + g >= limit[nt][c & 1])
+                  x[nt][j][c] = -INFINITY;
+        }
+
+        // ---- running maximum: raised only when a logit passes it by the headroom
+        bool passes = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) passes |= x[nt][j][c] > top[nt][c & 1] + kHeadroom;
+        if (__any_sync(0xffffffffu, passes)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float m = fmaxf(fmaxf(x[nt][0][c], x[nt][0][c + 2]), fmaxf(x[nt][1][c], x[nt][1][c + 2]));
+              m = fmaxf(m, top[nt][c]);
+#pragma unroll
+              for (int s = 4; s < 32; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+              const float keep = exp2_approx(top[nt][c] - m);
+              top[nt][c] = m;
+              sum[nt][c] *= keep;
+              low[nt][c] *= keep;
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  o[nt][gr][k >> 1][k & 1][c] *= keep;
+                  o[nt][gr][k >> 1][k & 1][c + 2] *= keep;
+                }
+            }
+        }
+
+        // ---- weights, as columns of the second product
+        uint32_t weight[NT][kWeights][2][2];  // part, matrix step j, half h
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float a = exp2_approx(x[nt][j][2 * h] - top[nt][0] + kWeightLog2);
+              const float c = exp2_approx(x[nt][j][2 * h + 1] - top[nt][1] + kWeightLog2);
+              sum[nt][0] += a;
+              sum[nt][1] += c;
+              const uint32_t high = pack_half2(a, c);
+              weight[nt][0][j][h] = transpose8(high);
+              if constexpr (kWeights == 2) {
+                const float2 f = half2_floats(high);
+                weight[nt][1][j][h] = transpose8(pack_half2(a - f.x, c - f.y));
+              }
+            }
+
+        // ---- value scales: pairs of tokens (16 j + 8 h + 2 t, + 1)
+        uint32_t step[NG][2][2], minimum[2][2];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const uint4 w =
+              *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + gr * 64 + t * 16);
+          step[gr][0][0] = w.x;
+          step[gr][0][1] = w.y;
+          step[gr][1][0] = w.z;
+          step[gr][1][1] = w.w;
+        }
+        {
+          const uint4 w = *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + kDim +
+                                                          min(g, NG - 1) * 64 + t * 16);
+          minimum[0][0] = g < NG ? w.x : 0u;
+          minimum[0][1] = g < NG ? w.y : 0u;
+          minimum[1][0] = g < NG ? w.z : 0u;
+          minimum[1][1] = g < NG ? w.w : 0u;
+        }
+        if (held < kBlockTokens) {  // rows that are not held: nothing of them may enter a product
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = 16 * j + 8 * h + 2 * t;
+              const uint32_t keep = (r < held ? 0xffffu : 0u) | (r + 1 < held ? 0xffff0000u : 0u);
+              minimum[j][h] &= keep;
+#pragma unroll
+              for (int gr = 0; gr < NG; ++gr) step[gr][j][h] &= keep;
+            }
+        }
+        uint32_t most = 0;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          most = hmax2(most, hmax2(hmax2(step[gr][0][0], step[gr][0][1]),
+                                   hmax2(step[gr][1][0], step[gr][1][1])));
+        most = hmax2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = hmax2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int most_log2 = static_cast<int>(max(most >> 10 & 31u, most >> 26 & 31u)) - 14;
+        if (most_log2 > step_log2) {  // the same in every lane
+          const float keep = step_log2 < -32 ? 0.0f : exp2_approx(static_cast<float>(step_log2 - most_log2));
+          step_log2 = most_log2;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[nt][gr][k >> 1][k & 1][c] *= keep;
+        }
+        const __half2 unit = __half2half2(__float2half_rn(exp2_approx(static_cast<float>(-step_log2))));
+        const uint32_t unit_bits = *reinterpret_cast<const uint32_t*>(&unit);
+
+        // ---- weighted minima: row g of the operand, what rounding the centred
+        // ones to FP16 lost in row g + 8
+        uint32_t rest[2][2] = {{0u, 0u}, {0u, 0u}};
+        float low_unit = 1.0f;
+        if constexpr (kCentred) {
+          // minimum + 8 step as an unevaluated sum of two FP16 numbers (Knuth's
+          // two-sum), halved where 8 step could pass FP16's largest
+          const bool large = most_log2 > 12;
+          low_unit = large ? 2.0f : 1.0f;
+          const uint32_t eight = large ? 0x44004400u : 0x48004800u, one = large ? 0x38003800u : 0x3c003c00u;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t mine = step[0][j][h];
+#pragma unroll
+              for (int gr = 1; gr < NG; ++gr) mine = g == gr ? step[gr][j][h] : mine;
+              const uint32_t a = hmul2(g < NG ? mine : 0u, eight), c = hmul2(minimum[j][h], one);
+              const uint32_t all = hadd2(a, c), back = hsub2(all, a);
+              rest[j][h] = hadd2(hsub2(a, hsub2(all, back)), hsub2(c, back));
+              minimum[j][h] = all;
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int part = 0; part < kWeights; ++part)
+              mma16816(acc, minimum[j][0], rest[j][0], minimum[j][1], rest[j][1],
+                       weight[nt][part][j][0], weight[nt][part][j][1]);
+          low[nt][0] = kCentred ? fmaf(acc[0] + acc[2], low_unit, low[nt][0]) : low[nt][0] + acc[0];
+          low[nt][1] = kCentred ? fmaf(acc[1] + acc[3], low_unit, low[nt][1]) : low[nt][1] + acc[1];
+        }
+        // ---- weighted codes
+        uint32_t word[2][2][2 * NG];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint8_t* from =
+                entry + kv4_value_codes(kDim) + (8 * j + 4 * h + t) * kDim + 8 * NG * g;
+            if constexpr (NG == 1) {
+              const uint2 w = *reinterpret_cast<const uint2*>(from);
+              word[j][h][0] = w.x;
+              word[j][h][1] = w.y;
+            } else {
+#pragma unroll
+              for (int k = 0; k < NG / 2; ++k) {
+                const uint4 w = *reinterpret_cast<const uint4*>(from + 16 * k);
+                word[j][h][4 * k] = w.x;
+                word[j][h][4 * k + 1] = w.y;
+                word[j][h][4 * k + 2] = w.z;
+                word[j][h][4 * k + 3] = w.w;
+              }
+            }
+          }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          uint32_t scaled[NT][kWeights][2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t s = hmul2(step[gr][j][h], unit_bits);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                scaled[nt][0][j][h] = hmul2(weight[nt][0][j][h], s);
+                if constexpr (kWeights == 2)  // what the first part's rounding lost, and the rest
+                  scaled[nt][1][j][h] =
+                      hfma2(weight[nt][1][j][h], s,
+                            hfma2(weight[nt][0][j][h], s, scaled[nt][0][j][h] ^ 0x80008000u));
+              }
+            }
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const uint32_t r0 = word[j][0][2 * gr + w] >> (8 * s);
+                  const uint32_t r1 = word[j][1][2 * gr + w] >> (8 * s);
+#pragma unroll
+                  for (int part = 0; part < kWeights; ++part)
+                    mma16816(acc, even_codes<kCentred>(r0), odd_codes<kCentred>(r0),
+                             even_codes<kCentred>(r1), odd_codes<kCentred>(r1),
+                             scaled[nt][part][j][0], scaled[nt][part][j][1]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[nt][gr][w][s][c] += acc[c];
+              }
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      fetch(i + kStages, stage);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    cp_async_wait<0>();
+
+    // ---- the segment's result
+    const bool whole = count == n;
+    const int64_t part = range * 2 + (at == range * quota ? 0 : 1);
+    const float code_unit = exp2f(static_cast<float>((kCentred ? 0 : 24) + max(step_log2, -32)));
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float s = sum[nt][c];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        const int r = nt * 8 + 2 * t + c;
+        const float scale = whole ? (s != 0.0f ? 1.0f / s : 0.0f) : 1.0f;
+        const int row = row0 + r;
+        const int64_t out_row =
+            (static_cast<int64_t>(b) * p.new_tokens + row / p.group) * p.query_heads +
+            static_cast<int64_t>(kv_head) * p.group + row % p.group;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const float minima = __shfl_sync(0xffffffffu, low[nt][c], gr * 4 + t);
+          float y[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float* acc = o[nt][gr][k >> 1][k & 1];
+            y[2 * k] = fmaf(acc[c], code_unit, minima) * scale;
+            y[2 * k + 1] = fmaf(acc[c + 2], code_unit * 0.0625f, minima) * scale;
+          }
+          if (row_live[nt][c]) {
+            if (whole)
+              store8(p.out, out_row * kDim + 64 * gr + 8 * g, p.out_type, y);
+            else
+              store8(p.part_o, (part * kTile + r) * kDim + 64 * gr + 8 * g, SA_TYPE_F32, y);
+          }
+        }
+        if (g == 0 && row_live[nt][c]) {
+          if (!whole) {
+            p.part_ml[(part * kTile + r) * 2] = top[nt][c];
+            p.part_ml[(part * kTile + r) * 2 + 1] = s;
+          } else if (p.lse) {
+            p.lse[out_row] =
+                s != 0.0f ? (top[nt][c] - kWeightLog2 + log2f(s)) * 0.6931471805599453f : -INFINITY;
+          }
+        }
+      }
+    at += count;
   }
-  if (lane == 0) {
-    part[warp][0] = top;
-    part[warp][1] = sum;
+}
+
+// Joins the parts of split units and writes the rows of empty ones: one CTA a
+// unit, a warp a query row.
+template <int NG>
+__global__ void __launch_bounds__(256) merge_kernel(const Kv4AttnParams p, int tile) {
+  constexpr int kDim = 64 * NG, kPerLane = kDim / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int list = blockIdx.x / p.units_per_list, unit = blockIdx.x % p.units_per_list;
+  pdl_wait();
+  const int start = p.starts[list], n = p.starts[list + 1] - start;
+  const int64_t entries =
+      static_cast<int64_t>(p.starts[p.requests * p.lists_per_request]) * p.units_per_list;
+  const int64_t quota = quota_of(entries, static_cast<int64_t>(p.ctas) * kWarps);
+  const int64_t begin = static_cast<int64_t>(start) * p.units_per_list + static_cast<int64_t>(unit) * n;
+  const int64_t from = begin / quota, to = n ? (begin + n - 1) / quota : from;
+  if (n && from == to) return;  // written by its warp
+  const int b = list / p.lists_per_request;
+  const int kv_head =
+      list % p.lists_per_request * (p.kv_heads / p.lists_per_request) + unit / p.row_tiles;
+  const int row0 = unit % p.row_tiles * tile;
+  for (int r = warp; r < tile && row0 + r < p.rows; r += 8) {
+    float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
+    if (n) {
+      // The range of part k begins inside the unit, or (the first) before it.
+      auto slot = [&](int64_t k) { return (k * 2 + (k * quota >= begin ? 0 : 1)) * tile + r; };
+      for (int64_t k = from + lane; k <= to; k += 32) top = fmaxf(top, p.part_ml[slot(k) * 2]);
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+#pragma unroll 4
+      for (int64_t k = from; k <= to; ++k) {
+        const int64_t at = slot(k);
+        const float w = exp2_approx(p.part_ml[at * 2] - top);
+        sum = fmaf(w, p.part_ml[at * 2 + 1], sum);
+#pragma unroll
+        for (int j = 0; j < kPerLane; ++j)
+          o[j] = fmaf(w, p.part_o[at * kDim + j * 32 + lane], o[j]);
+      }
+    }
+    const int row = row0 + r;
+    const int64_t out_row =
+        (static_cast<int64_t>(b) * p.new_tokens + row / p.group) * p.query_heads +
+        static_cast<int64_t>(kv_head) * p.group + row % p.group;
+    const float scale = sum != 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) {
+      const int64_t e = out_row * kDim + j * 32 + lane;
+      const float y = o[j] * scale;
+      if (p.out_type == SA_TYPE_F32)
+        static_cast<float*>(p.out)[e] = y;
+      else if (p.out_type == SA_TYPE_F16)
+        static_cast<__half*>(p.out)[e] = __float2half_rn(y);
+      else
+        static_cast<__nv_bfloat16*>(p.out)[e] = __float2bfloat16_rn(y);
+    }
+    if (p.lse && lane == 0)
+      p.lse[out_row] =
+          sum != 0.0f ? (top - kWeightLog2 + log2f(sum)) * 0.6931471805599453f : -INFINITY;
   }
-  for (int j = 0; j < per_lane; ++j) part[warp][2 + lane * per_lane + j] = o[j];
-  __syncthreads();
-  float all_top = -INFINITY, all_sum = 0.0f;
-  for (int w = 0; w < kWarps; ++w) all_top = fmaxf(all_top, part[w][0]);
-  for (int w = 0; w < kWarps; ++w)
-    if (part[w][1] != 0.0f) all_sum += part[w][1] * expf(part[w][0] - all_top);
-  for (int e = threadIdx.x; e < d; e += blockDim.x) {
-    float value = 0.0f;
-    for (int w = 0; w < kWarps; ++w)
-      if (part[w][1] != 0.0f) value += part[w][2 + e] * expf(part[w][0] - all_top);
-    store_from_float(p.out, static_cast<int64_t>(row) * d + e, p.out_type,
-                     all_sum != 0.0f ? value / all_sum : 0.0f);
+}
+
+// ---- host ---------------------------------------------------------------------------------
+
+// Query rows of a unit: 16 where a KV head has more than 8 and registers allow
+// (BF16 and FP16 at head_dim up to 128), else 8.
+int tile_rows(size_t rows, size_t head_dim, int query_type) {
+  return rows > 8 && head_dim <= 128 && query_type != SA_TYPE_F32 ? 16 : 8;
+}
+
+int max_warps(size_t head_dim, int tile) {
+  return device_sm_count() * (head_dim <= 128 && tile == 8 ? 2 : 1) * kWarps;
+}
+
+size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
+
+template <int NG, int NT, int MODE>
+sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
+  static int configured[kMaxDevices];
+  const auto kernel = attention_kernel<NG, NT, MODE>;
+  constexpr int kMost = Ring<NG>::kBytes + (kMaxLists + 1) * (int)sizeof(int);
+  const sa_status st = ensure_smem_limit(reinterpret_cast<const void*>(kernel), kMost, configured);
+  if (st != SA_OK) return st;
+  const size_t smem = Ring<NG>::kBytes + (size_t)(lists + 1) * sizeof(int);
+  SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(kWarps * 32), smem, stream, false, p));
+  return cuda_status(launch_kernel(merge_kernel<NG>, dim3(lists * p.units_per_list), dim3(256), 0,
+                                   stream, true, p, 8 * NT),
+                     "attention_kv4 merge launch");
+}
+
+template <int NG>
+sa_status launch_dim(const Kv4AttnParams& p, int lists, int tile, cudaStream_t stream) {
+  const int mode = p.query_type == SA_TYPE_F32 ? 2 : p.out_type == SA_TYPE_F16 ? 1 : 0;
+  if constexpr (NG <= 2) {
+    if (tile == 16)
+      return mode == 0 ? launch<NG, 2, 0>(p, lists, stream) : launch<NG, 2, 1>(p, lists, stream);
   }
-  if (p.lse && threadIdx.x == 0)
-    p.lse[row] = all_sum != 0.0f ? all_top + logf(all_sum) : -INFINITY;
+  return mode == 0   ? launch<NG, 1, 0>(p, lists, stream)
+         : mode == 1 ? launch<NG, 1, 1>(p, lists, stream)
+                     : launch<NG, 1, 2>(p, lists, stream);
 }
 
 bool known_type(int type) {
@@ -174,7 +882,11 @@ extern "C" SA_API size_t sa_attention_kv4_workspace_size(size_t requests, size_t
   if (requests == 0 || new_tokens == 0 || kv_heads == 0 || query_heads == 0 ||
       query_heads % kv_heads != 0 || sa_kv4_entry_bytes(head_dim) == 0)
     return 0;
-  return 256;
+  // starts of up to kMaxLists lists, two parts a warp: the same bytes for 8
+  // rows on twice the warps as for 16
+  const size_t rows = (size_t)max_warps(head_dim, 8) * 2 * 8;
+  return round256((kMaxLists + 1) * sizeof(int)) + rows * 2 * sizeof(float) +
+         rows * head_dim * sizeof(float);
 }
 
 extern "C" SA_API sa_status sa_attention_kv4(
@@ -196,27 +908,30 @@ extern "C" SA_API sa_status sa_attention_kv4(
     return fail(SA_ERR_UNSUPPORTED, "attention_kv4: a 16-bit query gives an output of its own type");
   if (sa_kv4_entry_bytes(head_dim) == 0)
     return fail(SA_ERR_UNSUPPORTED, "attention_kv4: head_dim must be 64, 128 or 256");
-  if ((reinterpret_cast<uintptr_t>(pool) & 15u) != 0)
-    return fail(SA_ERR_INVALID_ARG, "attention_kv4: the pool must be 16-byte aligned");
-  size_t lists = 1;
+  if ((reinterpret_cast<uintptr_t>(pool) & 15u) != 0 || (reinterpret_cast<uintptr_t>(out) & 15u) != 0)
+    return fail(SA_ERR_INVALID_ARG, "attention_kv4: the pool and out must be 16-byte aligned");
+  size_t lists = 1, list_blocks = table_blocks;
   if (selected) {
     if (!selected_count || budget == 0 || select_groups == 0 || kv_heads % select_groups != 0)
       return fail(SA_ERR_INVALID_ARG, "attention_kv4: invalid selection");
     if (new_tokens != 1)
       return fail(SA_ERR_UNSUPPORTED, "attention_kv4: a selection serves one new token a request");
     lists = select_groups;
+    list_blocks = budget + 1;
   }
-  if (requests * lists > (size_t)kMaxLists || requests > (size_t)kMaxLists)
+  if (requests > (size_t)kMaxLists || lists > (size_t)kMaxLists || requests * lists > (size_t)kMaxLists)
     return fail(SA_ERR_UNSUPPORTED, "attention_kv4: more than 8192 requests or lists");
-  if (pool_blocks > 0x7fffffffu / kBlockTokens || table_blocks > 0x7fffffffu / kBlockTokens)
-    return fail(SA_ERR_UNSUPPORTED, "attention_kv4: more than 2^31 slots");
+  constexpr size_t kMost = 0x7fffffffu;
+  if (pool_blocks > kMost / kBlockTokens || table_blocks > kMost / kBlockTokens || budget >= kMost ||
+      requests * lists * list_blocks > kMost)
+    return fail(SA_ERR_UNSUPPORTED, "attention_kv4: more than 2^31 slots or listed blocks");
+  if (query_heads > kMost || new_tokens > kMost || requests * query_heads > kMost / new_tokens)
+    return fail(SA_ERR_UNSUPPORTED, "attention_kv4: too many query rows");
   const size_t need =
       sa_attention_kv4_workspace_size(requests, new_tokens, query_heads, kv_heads, head_dim);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
     return fail(SA_ERR_CAPACITY,
                 "attention_kv4: workspace unaligned or smaller than sa_attention_kv4_workspace_size()");
-  if (requests * new_tokens * query_heads > 0x7fffffffu)
-    return fail(SA_ERR_UNSUPPORTED, "attention_kv4: too many query rows");
   Kv4AttnParams p{};
   p.query = query;
   p.stride_request = stride_request;
@@ -240,9 +955,21 @@ extern "C" SA_API sa_status sa_attention_kv4(
   p.new_tokens = (int)new_tokens;
   p.query_heads = (int)query_heads;
   p.kv_heads = (int)kv_heads;
-  p.head_dim = (int)head_dim;
-  p.scale = scale;
-  attention_simple<<<(unsigned)(requests * new_tokens * query_heads), kWarps * 32, 0,
-                     static_cast<cudaStream_t>(stream)>>>(p);
-  return cuda_status(cudaGetLastError(), "attention_kv4 launch");
+  p.group = (int)(query_heads / kv_heads);
+  p.rows = p.group * p.new_tokens;
+  const int tile = tile_rows((size_t)p.rows, head_dim, query_type);
+  p.row_tiles = (p.rows + tile - 1) / tile;
+  p.units_per_list = (int)(kv_heads / lists) * p.row_tiles;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.ctas = max_warps(head_dim, tile) / kWarps;
+  const size_t part_rows = (size_t)p.ctas * kWarps * 2 * tile;
+  char* ws = static_cast<char*>(workspace);
+  p.starts = reinterpret_cast<int*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + round256((kMaxLists + 1) * sizeof(int)));
+  p.part_o = p.part_ml + part_rows * 2;
+  const int all = (int)(requests * lists);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return head_dim == 64    ? launch_dim<1>(p, all, tile, s)
+         : head_dim == 128 ? launch_dim<2>(p, all, tile, s)
+                           : launch_dim<4>(p, all, tile, s);
 }
