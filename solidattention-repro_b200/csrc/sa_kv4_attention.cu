@@ -39,6 +39,7 @@
 // alone is written at once; parts of units go to the workspace as (max, sum,
 // weighted values) and merge_kernel joins them in list order.
 #include <algorithm>
+#include <type_traits>
 
 #include "sa_kv4.cuh"
 
@@ -215,6 +216,20 @@ struct Ring {
   static constexpr int kBytes = kWarps * kStages * kEntry;
 };
 
+// Stages are read with the lanes' fragment pattern, so 16-byte pieces are
+// permuted inside their rows on the way in: piece x of key row r, or of value
+// pair row r, goes to place x ^ swizzle. Eight consecutive lanes then read all
+// 32 banks (value reads took four passes without it: 145 -> 135 us for 64 x 8K
+// tokens).
+template <int NG>
+__device__ __forceinline__ int key_swizzle(int r) {
+  return NG == 4 ? r & 1 : 0;
+}
+template <int NG>
+__device__ __forceinline__ int value_swizzle(int r) {
+  return NG == 1 ? r & 2 : NG == 2 ? 2 * (r & 3) : (r & 1) | 2 * (r & 2);
+}
+
 template <int NG, int NT, int MODE>
 constexpr int min_ctas() {
   return NG <= 2 && NT == 1 ? 2 : 1;
@@ -321,8 +336,15 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
           uint8_t* to = ring + stage * kEntry;
 #pragma unroll
           for (int k = 0; k < (kPieces + 31) / 32; ++k) {
+            // 32 NG pieces of keys, 32 NG of values in rows of 2 NG and 4 NG
+            // pieces, then the scales
             const int piece = k * 32 + lane;
-            if (kPieces % 32 == 0 || piece < kPieces) cp_async16(to + piece * 16, from + piece * 16);
+            int place = piece;
+            if (k < 2 * NG)
+              place ^= key_swizzle<NG>(piece / (2 * NG));
+            else if (k < 4 * NG)
+              place ^= value_swizzle<NG>((piece - 64 * NG) / (4 * NG));
+            if (kPieces % 32 == 0 || piece < kPieces) cp_async16(to + place * 16, from + piece * 16);
           }
         }
       }
@@ -400,13 +422,14 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
 
     float o[NT][NG][2][2][4];  // codes' sums of element 64 gr + 8 g + 4 w + 2 s (+ 1, times 16)
     float low[NT][2];          // minima's sums: lane group g holds value group g's
-    float top[NT][2], sum[NT][2];
-    int step_log2 = -64;  // E: value steps are held as s * 2^-E
+    float base[NT][2], sum[NT][2];  // running maximum - 11; sum of 2^(x - base)
+    int step_log2 = 0;              // E: value steps are held as s * 2^-E
+    uint32_t step_bits = 0;         // 2^E as FP16 bits, 0 before the first block
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        top[nt][c] = -3.0e38f;
+        base[nt][c] = -3.0e38f;
         sum[nt][c] = 0.0f;
       }
 #pragma unroll
@@ -419,192 +442,176 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
           for (int c = 0; c < 4; ++c) o[nt][gr][m >> 1][m & 1][c] = 0.0f;
     }
 
-    int stage = 0;
-    for (int i = 0; i < count; ++i) {
-      cp_async_wait<kStages - 1>();
-      __syncwarp();
-      if (!(unread >> stage & 1)) {
-        const uint8_t* entry = ring + stage * kEntry;
-        const bool last = first + i == n - 1;
-        // first token of the block, in a dense list or the newest block
-        const int token0 = (ids ? newest : first + i) * kBlockTokens;
-        const int held = last ? length - newest * kBlockTokens : kBlockTokens;
-        const bool masked = (ids ? last : true) && token0 + kBlockTokens > least;
-
-        // ---- logits
-        float x[NT][2][4];
-        uint4 scales[NG];
+    // One entry: the block whose first token is token0, `held` of its rows in
+    // use. Blocks that every row sees whole take the copy without masks.
+    auto process = [&](const uint8_t* entry, int token0, int held, auto masks) {
+      constexpr bool kMasked = decltype(masks)::value;
+      // ---- logits
+      float x[NT][2][4];
+      uint4 scales[NG];  // (step, minimum) of rows g, g + 8, g + 16, g + 24
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-          scales[gr] = *reinterpret_cast<const uint4*>(entry + kv4_key_scales(kDim) + gr * 128 + g * 16);
+      for (int gr = 0; gr < NG; ++gr)
+        scales[gr] = *reinterpret_cast<const uint4*>(entry + kv4_key_scales(kDim) + gr * 128 + g * 16);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t word[2][2 * NG];
+      for (int j = 0; j < 2; ++j) {
+        uint32_t word[2][2 * NG];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint8_t* from = entry + (16 * j + 8 * h + g) * (kDim / 2) + 8 * NG * t;
-            if constexpr (NG == 1) {
-              const uint2 w = *reinterpret_cast<const uint2*>(from);
-              word[h][0] = w.x;
-              word[h][1] = w.y;
-            } else {
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* from = entry + (16 * j + 8 * h + g) * (kDim / 2);
+          if constexpr (NG == 1) {
+            const uint2 w = *reinterpret_cast<const uint2*>(from + 8 * t);
+            word[h][0] = w.x;
+            word[h][1] = w.y;
+          } else {
 #pragma unroll
-              for (int k = 0; k < NG / 2; ++k) {
-                const uint4 w = *reinterpret_cast<const uint4*>(from + 16 * k);
-                word[h][4 * k] = w.x;
-                word[h][4 * k + 1] = w.y;
-                word[h][4 * k + 2] = w.z;
-                word[h][4 * k + 3] = w.w;
-              }
+            for (int k = 0; k < NG / 2; ++k) {
+              const uint4 w = *reinterpret_cast<const uint4*>(
+                  from + 16 * ((NG / 2 * t + k) ^ key_swizzle<NG>(g)));
+              word[h][4 * k] = w.x;
+              word[h][4 * k + 1] = w.y;
+              word[h][4 * k + 2] = w.z;
+              word[h][4 * k + 3] = w.w;
             }
           }
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr) {
-            float acc[NT][kParts][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int part = 0; part < kParts; ++part)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[nt][part][c] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-              for (int s = 0; s < 2; ++s) {
-                const uint32_t r0 = word[0][2 * gr + w] >> (8 * s), r1 = word[1][2 * gr + w] >> (8 * s);
-                const uint32_t a0 = even_codes<kCentredKeys>(r0), a1 = even_codes<kCentredKeys>(r1),
-                               a2 = odd_codes<kCentredKeys>(r0), a3 = odd_codes<kCentredKeys>(r1);
-                const int k = (w * 2 + s) * 2;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int part = 0; part < kParts; ++part)
-                    mma16816(acc[nt][part], a0, a1, a2, a3, q[nt][part][gr][k], q[nt][part][gr][k + 1]);
-              }
-            const uint32_t sm0 = j == 0 ? scales[gr].x : scales[gr].z;
-            const uint32_t sm1 = j == 0 ? scales[gr].y : scales[gr].w;
-            float2 f0 = half2_floats(sm0), f1 = half2_floats(sm1);
-            if constexpr (kCentredKeys) {
-              f0.y = fmaf(8.0f, f0.x, f0.y);
-              f1.y = fmaf(8.0f, f1.x, f1.y);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const float step = c < 2 ? f0.x : f1.x, minimum = c < 2 ? f0.y : f1.y;
-                const float lowest = minimum * row_sum[nt][gr][c & 1];
-                const float dot =
-                    kParts == 2 ? acc[nt][0][c] + acc[nt][kParts - 1][c] : acc[nt][0][c];
-                const float term = fmaf(step * dot, row_factor[nt][c & 1], lowest);
-                x[nt][j][c] = gr == 0 ? term : x[nt][j][c] + term;
-              }
-          }
         }
-        if (masked) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                if (token0 + 16 * j + 8 * (c >> 1) + g >= limit[nt][c & 1])
-                  x[nt][j][c] = -INFINITY;
-        }
-
-        // ---- running maximum: raised only when a logit passes it by the headroom
-        bool passes = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) passes |= x[nt][j][c] > top[nt][c & 1] + kHeadroom;
-        if (__any_sync(0xffffffffu, passes)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float m = fmaxf(fmaxf(x[nt][0][c], x[nt][0][c + 2]), fmaxf(x[nt][1][c], x[nt][1][c + 2]));
-              m = fmaxf(m, top[nt][c]);
-#pragma unroll
-              for (int s = 4; s < 32; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
-              const float keep = exp2_approx(top[nt][c] - m);
-              top[nt][c] = m;
-              sum[nt][c] *= keep;
-              low[nt][c] *= keep;
-#pragma unroll
-              for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  o[nt][gr][k >> 1][k & 1][c] *= keep;
-                  o[nt][gr][k >> 1][k & 1][c + 2] *= keep;
-                }
-            }
-        }
-
-        // ---- weights, as columns of the second product
-        uint32_t weight[NT][kWeights][2][2];  // part, matrix step j, half h
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float a = exp2_approx(x[nt][j][2 * h] - top[nt][0] + kWeightLog2);
-              const float c = exp2_approx(x[nt][j][2 * h + 1] - top[nt][1] + kWeightLog2);
-              sum[nt][0] += a;
-              sum[nt][1] += c;
-              const uint32_t high = pack_half2(a, c);
-              weight[nt][0][j][h] = transpose8(high);
-              if constexpr (kWeights == 2) {
-                const float2 f = half2_floats(high);
-                weight[nt][1][j][h] = transpose8(pack_half2(a - f.x, c - f.y));
-              }
-            }
-
-        // ---- value scales: pairs of tokens (16 j + 8 h + 2 t, + 1)
-        uint32_t step[NG][2][2], minimum[2][2];
+        float lowest[NT][4];
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
-          const uint4 w =
-              *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + gr * 64 + t * 16);
-          step[gr][0][0] = w.x;
-          step[gr][0][1] = w.y;
-          step[gr][1][0] = w.z;
-          step[gr][1][1] = w.w;
+          float acc[NT][kParts][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[nt][part][c] = 0.0f;
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const uint32_t r0 = word[0][2 * gr + w] >> (8 * s), r1 = word[1][2 * gr + w] >> (8 * s);
+              const uint32_t a0 = even_codes<kCentredKeys>(r0), a1 = even_codes<kCentredKeys>(r1),
+                             a2 = odd_codes<kCentredKeys>(r0), a3 = odd_codes<kCentredKeys>(r1);
+              const int k = (w * 2 + s) * 2;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+                  mma16816(acc[nt][part], a0, a1, a2, a3, q[nt][part][gr][k], q[nt][part][gr][k + 1]);
+            }
+          const uint32_t sm0 = j == 0 ? scales[gr].x : scales[gr].z;
+          const uint32_t sm1 = j == 0 ? scales[gr].y : scales[gr].w;
+          float2 f0 = half2_floats(sm0), f1 = half2_floats(sm1);
+          if constexpr (kCentredKeys) {
+            f0.y = fmaf(8.0f, f0.x, f0.y);
+            f1.y = fmaf(8.0f, f1.x, f1.y);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float step = c < 2 ? f0.x : f1.x, minimum = c < 2 ? f0.y : f1.y;
+              const float dot =
+                  kParts == 2 ? acc[nt][0][c] + acc[nt][kParts - 1][c] : acc[nt][0][c];
+              x[nt][j][c] = gr == 0 ? step * dot : fmaf(step, dot, x[nt][j][c]);
+              lowest[nt][c] = gr == 0 ? minimum * row_sum[nt][gr][c & 1]
+                                      : fmaf(minimum, row_sum[nt][gr][c & 1], lowest[nt][c]);
+            }
         }
-        {
-          const uint4 w = *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + kDim +
-                                                          min(g, NG - 1) * 64 + t * 16);
-          minimum[0][0] = g < NG ? w.x : 0u;
-          minimum[0][1] = g < NG ? w.y : 0u;
-          minimum[1][0] = g < NG ? w.z : 0u;
-          minimum[1][1] = g < NG ? w.w : 0u;
-        }
-        if (held < kBlockTokens) {  // rows that are not held: nothing of them may enter a product
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            x[nt][j][c] = fmaf(x[nt][j][c], row_factor[nt][c & 1], lowest[nt][c]);
+      }
+      if constexpr (kMasked) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int r = 16 * j + 8 * h + 2 * t;
-              const uint32_t keep = (r < held ? 0xffffu : 0u) | (r + 1 < held ? 0xffff0000u : 0u);
-              minimum[j][h] &= keep;
+            for (int c = 0; c < 4; ++c)
+              if (token0 + 16 * j + 8 * (c >> 1) + g >= limit[nt][c & 1])
+                x[nt][j][c] = -INFINITY;
+      }
+
+      // ---- value scales: pairs of tokens (16 j + 8 h + 2 t, + 1)
+      uint32_t step[NG][2][2], minimum[2][2];
 #pragma unroll
-              for (int gr = 0; gr < NG; ++gr) step[gr][j][h] &= keep;
-            }
-        }
-        uint32_t most = 0;
+      for (int gr = 0; gr < NG; ++gr) {
+        const uint4 w =
+            *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + gr * 64 + t * 16);
+        step[gr][0][0] = w.x;
+        step[gr][0][1] = w.y;
+        step[gr][1][0] = w.z;
+        step[gr][1][1] = w.w;
+      }
+      {
+        const uint4 w = *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + kDim +
+                                                        min(g, NG - 1) * 64 + t * 16);
+        minimum[0][0] = g < NG ? w.x : 0u;
+        minimum[0][1] = g < NG ? w.y : 0u;
+        minimum[1][0] = g < NG ? w.z : 0u;
+        minimum[1][1] = g < NG ? w.w : 0u;
+      }
+      if constexpr (kMasked) {  // rows that are not held: nothing of them may enter a product
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-          most = hmax2(most, hmax2(hmax2(step[gr][0][0], step[gr][0][1]),
-                                   hmax2(step[gr][1][0], step[gr][1][1])));
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = 16 * j + 8 * h + 2 * t;
+            const uint32_t keep = (r < held ? 0xffffu : 0u) | (r + 1 < held ? 0xffff0000u : 0u);
+            minimum[j][h] &= keep;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) step[gr][j][h] &= keep;
+          }
+      }
+      // ---- running maxima of the logits and of the value steps, raised only
+      // when a logit passes its row's by the headroom or a step passes 2^E
+      uint32_t most = 0;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+        most = hmax2(most, hmax2(hmax2(step[gr][0][0], step[gr][0][1]),
+                                 hmax2(step[gr][1][0], step[gr][1][1])));
+      most &= 0x7fff7fffu;
+      bool passes = (most & 0xffffu) >= step_bits || most >> 16 >= step_bits;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          passes |= fmaxf(fmaxf(x[nt][0][c], x[nt][0][c + 2]), fmaxf(x[nt][1][c], x[nt][1][c + 2])) >
+                    base[nt][c] + (kHeadroom + kWeightLog2);
+      if (__any_sync(0xffffffffu, passes)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = fmaxf(fmaxf(x[nt][0][c], x[nt][0][c + 2]), fmaxf(x[nt][1][c], x[nt][1][c + 2]));
+            m -= kWeightLog2;
+            m = fmaxf(m, base[nt][c]);
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, s));
+            const float keep = exp2_approx(base[nt][c] - m);
+            base[nt][c] = m;
+            sum[nt][c] *= keep;
+            low[nt][c] *= keep;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                o[nt][gr][k >> 1][k & 1][c] *= keep;
+                o[nt][gr][k >> 1][k & 1][c + 2] *= keep;
+              }
+          }
         most = hmax2(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = hmax2(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int most_log2 = static_cast<int>(max(most >> 10 & 31u, most >> 26 & 31u)) - 14;
-        if (most_log2 > step_log2) {  // the same in every lane
-          const float keep = step_log2 < -32 ? 0.0f : exp2_approx(static_cast<float>(step_log2 - most_log2));
-          step_log2 = most_log2;
+        const uint32_t largest = max(most & 0xffffu, most >> 16);
+        if (largest >= step_bits) {  // the same in every lane
+          // steps stay as they are while the largest is in [2^-8, 1)
+          int exponent = static_cast<int>(largest >> 10) - 14;
+          if (exponent > -8 && exponent <= 0) exponent = 0;
+          const float keep = step_bits == 0 ? 0.0f : exp2_approx(static_cast<float>(step_log2 - exponent));
+          step_log2 = exponent;
+          step_bits = static_cast<uint32_t>(exponent + 15) << 10;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -614,105 +621,151 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[nt][gr][k >> 1][k & 1][c] *= keep;
         }
+      }
+      uint32_t scaled_step[NG][2][2];
+      {
         const __half2 unit = __half2half2(__float2half_rn(exp2_approx(static_cast<float>(-step_log2))));
         const uint32_t unit_bits = *reinterpret_cast<const uint32_t*>(&unit);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            scaled_step[gr][k >> 1][k & 1] = step_log2 == 0
+                                                 ? step[gr][k >> 1][k & 1]
+                                                 : hmul2(step[gr][k >> 1][k & 1], unit_bits);
+      }
 
-        // ---- weighted minima: row g of the operand, what rounding the centred
-        // ones to FP16 lost in row g + 8
-        uint32_t rest[2][2] = {{0u, 0u}, {0u, 0u}};
-        float low_unit = 1.0f;
-        if constexpr (kCentred) {
-          // minimum + 8 step as an unevaluated sum of two FP16 numbers (Knuth's
-          // two-sum), halved where 8 step could pass FP16's largest
-          const bool large = most_log2 > 12;
-          low_unit = large ? 2.0f : 1.0f;
-          const uint32_t eight = large ? 0x44004400u : 0x48004800u, one = large ? 0x38003800u : 0x3c003c00u;
+      // ---- weights, as columns of the second product
+      uint32_t weight[NT][kWeights][2][2];  // part, matrix step j, half h
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t mine = step[0][j][h];
-#pragma unroll
-              for (int gr = 1; gr < NG; ++gr) mine = g == gr ? step[gr][j][h] : mine;
-              const uint32_t a = hmul2(g < NG ? mine : 0u, eight), c = hmul2(minimum[j][h], one);
-              const uint32_t all = hadd2(a, c), back = hsub2(all, a);
-              rest[j][h] = hadd2(hsub2(a, hsub2(all, back)), hsub2(c, back));
-              minimum[j][h] = all;
-            }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int part = 0; part < kWeights; ++part)
-              mma16816(acc, minimum[j][0], rest[j][0], minimum[j][1], rest[j][1],
-                       weight[nt][part][j][0], weight[nt][part][j][1]);
-          low[nt][0] = kCentred ? fmaf(acc[0] + acc[2], low_unit, low[nt][0]) : low[nt][0] + acc[0];
-          low[nt][1] = kCentred ? fmaf(acc[1] + acc[3], low_unit, low[nt][1]) : low[nt][1] + acc[1];
-        }
-        // ---- weighted codes
-        uint32_t word[2][2][2 * NG];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint8_t* from =
-                entry + kv4_value_codes(kDim) + (8 * j + 4 * h + t) * kDim + 8 * NG * g;
-            if constexpr (NG == 1) {
-              const uint2 w = *reinterpret_cast<const uint2*>(from);
-              word[j][h][0] = w.x;
-              word[j][h][1] = w.y;
-            } else {
+            const float a = exp2_approx(x[nt][j][2 * h] - base[nt][0]);
+            const float c = exp2_approx(x[nt][j][2 * h + 1] - base[nt][1]);
+            sum[nt][0] += a;
+            sum[nt][1] += c;
+            const uint32_t high = pack_half2(a, c);
+            weight[nt][0][j][h] = transpose8(high);
+            if constexpr (kWeights == 2) {
+              const float2 f = half2_floats(high);
+              weight[nt][1][j][h] = transpose8(pack_half2(a - f.x, c - f.y));
+            }
+          }
+
+      // ---- weighted minima: row g of the operand, what rounding the centred
+      // ones to FP16 lost in row g + 8
+      uint32_t rest[2][2] = {{0u, 0u}, {0u, 0u}};
+      float low_unit = 1.0f;
+      if constexpr (kCentred) {
+        // minimum + 8 step as an unevaluated sum of two FP16 numbers (Knuth's
+        // two-sum), halved where 8 step could pass FP16's largest
+        const bool large = step_log2 > 12;
+        low_unit = large ? 2.0f : 1.0f;
+        const uint32_t eight = large ? 0x44004400u : 0x48004800u, one = large ? 0x38003800u : 0x3c003c00u;
 #pragma unroll
-              for (int k = 0; k < NG / 2; ++k) {
-                const uint4 w = *reinterpret_cast<const uint4*>(from + 16 * k);
-                word[j][h][4 * k] = w.x;
-                word[j][h][4 * k + 1] = w.y;
-                word[j][h][4 * k + 2] = w.z;
-                word[j][h][4 * k + 3] = w.w;
-              }
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t mine = step[0][j][h];
+#pragma unroll
+            for (int gr = 1; gr < NG; ++gr) mine = g == gr ? step[gr][j][h] : mine;
+            const uint32_t a = hmul2(g < NG ? mine : 0u, eight), c = hmul2(minimum[j][h], one);
+            const uint32_t all = hadd2(a, c), back = hsub2(all, a);
+            rest[j][h] = hadd2(hsub2(a, hsub2(all, back)), hsub2(c, back));
+            minimum[j][h] = all;
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int part = 0; part < kWeights; ++part)
+            mma16816(acc, minimum[j][0], rest[j][0], minimum[j][1], rest[j][1],
+                     weight[nt][part][j][0], weight[nt][part][j][1]);
+        low[nt][0] = kCentred ? fmaf(acc[0] + acc[2], low_unit, low[nt][0]) : low[nt][0] + acc[0];
+        low[nt][1] = kCentred ? fmaf(acc[1] + acc[3], low_unit, low[nt][1]) : low[nt][1] + acc[1];
+      }
+      // ---- weighted codes
+      uint32_t word[2][2][2 * NG];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t* from = entry + kv4_value_codes(kDim) + (8 * j + 4 * h + t) * kDim;
+          if constexpr (NG == 1) {
+            const uint2 w = *reinterpret_cast<const uint2*>(
+                from + 16 * ((g >> 1) ^ value_swizzle<NG>(t)) + 8 * (g & 1));
+            word[j][h][0] = w.x;
+            word[j][h][1] = w.y;
+          } else {
+#pragma unroll
+            for (int k = 0; k < NG / 2; ++k) {
+              const uint4 w = *reinterpret_cast<const uint4*>(
+                  from + 16 * ((NG / 2 * g + k) ^ value_swizzle<NG>(t)));
+              word[j][h][4 * k] = w.x;
+              word[j][h][4 * k + 1] = w.y;
+              word[j][h][4 * k + 2] = w.z;
+              word[j][h][4 * k + 3] = w.w;
+            }
+          }
+        }
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        uint32_t scaled[NT][kWeights][2][2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t s = scaled_step[gr][j][h];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              scaled[nt][0][j][h] = hmul2(weight[nt][0][j][h], s);
+              if constexpr (kWeights == 2)  // what the first part's rounding lost, and the rest
+                scaled[nt][1][j][h] =
+                    hfma2(weight[nt][1][j][h], s,
+                          hfma2(weight[nt][0][j][h], s, scaled[nt][0][j][h] ^ 0x80008000u));
             }
           }
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          uint32_t scaled[NT][kWeights][2][2];
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t s = hmul2(step[gr][j][h], unit_bits);
+            for (int nt = 0; nt < NT; ++nt) {
+              float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                scaled[nt][0][j][h] = hmul2(weight[nt][0][j][h], s);
-                if constexpr (kWeights == 2)  // what the first part's rounding lost, and the rest
-                  scaled[nt][1][j][h] =
-                      hfma2(weight[nt][1][j][h], s,
-                            hfma2(weight[nt][0][j][h], s, scaled[nt][0][j][h] ^ 0x80008000u));
+              for (int j = 0; j < 2; ++j) {
+                const uint32_t r0 = word[j][0][2 * gr + w] >> (8 * s);
+                const uint32_t r1 = word[j][1][2 * gr + w] >> (8 * s);
+#pragma unroll
+                for (int part = 0; part < kWeights; ++part)
+                  mma16816(acc, even_codes<kCentred>(r0), odd_codes<kCentred>(r0),
+                           even_codes<kCentred>(r1), odd_codes<kCentred>(r1),
+                           scaled[nt][part][j][0], scaled[nt][part][j][1]);
               }
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nt][gr][w][s][c] += acc[c];
             }
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  const uint32_t r0 = word[j][0][2 * gr + w] >> (8 * s);
-                  const uint32_t r1 = word[j][1][2 * gr + w] >> (8 * s);
-#pragma unroll
-                  for (int part = 0; part < kWeights; ++part)
-                    mma16816(acc, even_codes<kCentred>(r0), odd_codes<kCentred>(r0),
-                             even_codes<kCentred>(r1), odd_codes<kCentred>(r1),
-                             scaled[nt][part][j][0], scaled[nt][part][j][1]);
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[nt][gr][w][s][c] += acc[c];
-              }
-        }
+      }
+    };
+
+    int stage = 0;
+    for (int i = 0; i < count; ++i) {
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      if (!(unread >> stage & 1)) {
+        const uint8_t* entry = ring + stage * kEntry;
+        const int logical = ids ? newest : first + i;  // with ids, used for the newest block only
+        const int token0 = logical * kBlockTokens;
+        if ((!ids || first + i == n - 1) && token0 + kBlockTokens > least)
+          process(entry, token0, min(length - token0, kBlockTokens), std::true_type{});
+        else
+          process(entry, token0, kBlockTokens, std::false_type{});
       }
       __syncwarp();  // every lane has read the stage
       fetch(i + kStages, stage);
@@ -723,7 +776,7 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
     // ---- the segment's result
     const bool whole = count == n;
     const int64_t part = range * 2 + (at == range * quota ? 0 : 1);
-    const float code_unit = exp2f(static_cast<float>((kCentred ? 0 : 24) + max(step_log2, -32)));
+    const float code_unit = exp2f(static_cast<float>((kCentred ? 0 : 24) + step_log2));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -756,11 +809,11 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         }
         if (g == 0 && row_live[nt][c]) {
           if (!whole) {
-            p.part_ml[(part * kTile + r) * 2] = top[nt][c];
+            p.part_ml[(part * kTile + r) * 2] = base[nt][c];
             p.part_ml[(part * kTile + r) * 2 + 1] = s;
           } else if (p.lse) {
             p.lse[out_row] =
-                s != 0.0f ? (top[nt][c] - kWeightLog2 + log2f(s)) * 0.6931471805599453f : -INFINITY;
+                s != 0.0f ? (base[nt][c] + log2f(s)) * 0.6931471805599453f : -INFINITY;
           }
         }
       }
@@ -823,7 +876,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const Kv4AttnParams p, int t
     }
     if (p.lse && lane == 0)
       p.lse[out_row] =
-          sum != 0.0f ? (top - kWeightLog2 + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+          sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
   }
 }
 
