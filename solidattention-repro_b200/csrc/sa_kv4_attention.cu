@@ -34,10 +34,12 @@
 // by a warp vanish next to it.
 //
 // Work split. All (list, KV head, row tile) units' entries form one flat list;
-// every warp takes an equal contiguous range of it, whatever the lengths, and
-// streams its entries through a ring of its own. A unit that a warp covers
-// alone is written at once; parts of units go to the workspace as (max, sum,
-// weighted values) and merge_kernel joins them in list order.
+// every CTA takes an equal contiguous range of it, whatever the lengths, and
+// its warps equal contiguous parts of that, each streaming its entries through
+// a ring of its own. A unit that a warp covers alone is written at once. Parts
+// of units go to the workspace as (maximum, sum, weighted values), joined by
+// the CTA first where its whole range lies in one unit, and merge_kernel joins
+// them in the order of the list.
 #include <algorithm>
 #include <type_traits>
 
@@ -47,7 +49,8 @@ namespace sa {
 namespace {
 
 constexpr int kMaxLists = 8192;
-constexpr int kWarps = 8;        // of a CTA
+constexpr int kWarps = 8;        // of an attention CTA
+constexpr int kMergeWarps = 4, kMergeUnroll = 4;
 constexpr float kHeadroom = 4.0f;  // log2 by which a weight may exceed its row's running maximum
 constexpr float kWeightLog2 = 11.0f;  // weights are held as 2^11 p: at most 2^15 in FP16
 
@@ -71,18 +74,13 @@ struct Kv4AttnParams {
   int units_per_list;  // KV heads of a list * row_tiles
   float scale_log2;    // softmax scale * log2(e)
   int ctas;            // of the attention grid
+  int vector_rows;     // query rows are 16-byte aligned
   int* starts;         // workspace: [lists + 1] entries of the lists before each
   float* part_ml;      // workspace: [warps][2][rows of a tile][max, sum]
   float* part_o;       // workspace: [warps][2][rows of a tile][head_dim]
 };
 
 // ---- elements of the calls' types ------------------------------------------------
-
-__device__ __forceinline__ float load_as_float(const void* base, int64_t i, int type) {
-  if (type == SA_TYPE_F32) return static_cast<const float*>(base)[i];
-  if (type == SA_TYPE_F16) return __half2float(static_cast<const __half*>(base)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
-}
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -111,6 +109,19 @@ __device__ __forceinline__ void store8(void* base, int64_t i, int type, const fl
   }
 }
 
+// Four of them (a multiple of 4).
+__device__ __forceinline__ void store4(void* base, int64_t i, int type, float a, float b, float c,
+                                       float d) {
+  if (type == SA_TYPE_F32)
+    *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = make_float4(a, b, c, d);
+  else if (type == SA_TYPE_F16)
+    *reinterpret_cast<uint2*>(static_cast<__half*>(base) + i) =
+        make_uint2(pack_half2(a, b), pack_half2(c, d));
+  else
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(base) + i) =
+        make_uint2(pack_bf162(a, b), pack_bf162(c, d));
+}
+
 // ---- matrix fragments -------------------------------------------------------------
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -134,6 +145,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// 2^k, -126 <= k <= 127.
+__device__ __forceinline__ float power_of_2(int k) { return __int_as_float((k + 127) << 23); }
+
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -141,10 +155,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
                             *reinterpret_cast<const __half2*>(&c));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
@@ -172,7 +182,18 @@ __device__ __forceinline__ uint32_t odd_codes(uint32_t word) {
   return CENTRED ? hadd2((word & kNibble1) | 0x64006400u, 0xe480e480u) : word & kNibble1;
 }
 
+// ln(sum * 2^base); -inf for an empty row.
+__device__ __forceinline__ float log_of_sum(float base, float sum) {
+  return sum != 0.0f ? (base + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+}
+
 // ---- lists and units ----------------------------------------------------------------
+
+// Row of the output of query row `row` of a KV head.
+__device__ __forceinline__ int64_t output_row(const Kv4AttnParams& p, int b, int kv_head, int row) {
+  return (static_cast<int64_t>(b) * p.new_tokens + row / p.group) * p.query_heads +
+         static_cast<int64_t>(kv_head) * p.group + row % p.group;
+}
 
 // A request's length, 0 when it is out of range.
 __device__ __forceinline__ int checked_length(int length, int table_blocks) {
@@ -202,9 +223,48 @@ __device__ __forceinline__ int list_of(const int* starts, int lists, int at) {
   return low;
 }
 
-// Flat entries a warp takes.
-__device__ __forceinline__ int64_t quota_of(int64_t entries, int64_t warps) {
-  return max((entries + warps - 1) / warps, static_cast<int64_t>(1));
+// The ranges of the flat list: `cta` entries for each CTA, `warp` of them for
+// each of its warps.
+struct Quota {
+  int entries, cta, warp;
+};
+__device__ __forceinline__ Quota quota_of(int entries, int ctas) {
+  Quota q;
+  q.entries = entries;
+  q.cta = max((entries + ctas - 1) / ctas, 1);
+  q.warp = (q.cta + kWarps - 1) / kWarps;
+  return q;
+}
+
+// 16 elements as FP32.
+template <int TYPE>
+__device__ __forceinline__ void load16(const void* base, int64_t at, bool vectors, float (&x)[16]) {
+  using Element = Kv4Type<TYPE>;
+  const auto* from = static_cast<const typename Element::T*>(base) + at;
+  if (vectors) {
+    constexpr int kEach = 16 / sizeof(typename Element::T);
+#pragma unroll
+    for (int k = 0; k < 16 / kEach; ++k) {
+      const uint4 v = reinterpret_cast<const uint4*>(from)[k];
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (TYPE == SA_TYPE_F32) {
+          x[4 * k + i] = __uint_as_float(w[i]);
+        } else if constexpr (TYPE == SA_TYPE_BF16) {
+          x[8 * k + 2 * i] = __uint_as_float(w[i] << 16);
+          x[8 * k + 2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          x[8 * k + 2 * i] = f.x;
+          x[8 * k + 2 * i + 1] = f.y;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = Element::load(from[i]);
+  }
 }
 
 // ---- attention -------------------------------------------------------------------------
@@ -213,7 +273,9 @@ template <int NG>
 struct Ring {
   static constexpr int kEntry = 36 * 64 * NG;
   static constexpr int kStages = NG == 4 ? 2 : 3;
-  static constexpr int kBytes = kWarps * kStages * kEntry;
+  static constexpr int kStage = kEntry + 16;  // 16 zero bytes: the minima of lanes without a group
+  static constexpr int kWarpBytes = kStages * kStage;
+  static constexpr int kBytes = kWarps * kWarpBytes;
 };
 
 // Stages are read with the lanes' fragment pattern, so 16-byte pieces are
@@ -247,15 +309,19 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
   constexpr bool kCentred = kWeights == 2;    // value codes as c - 8
   constexpr bool kCentredKeys = kParts == 2;  // key codes too
   constexpr int kPieces = kEntry / 16;        // 16-byte pieces of an entry
+  constexpr int kStage = Ring<NG>::kStage;
+  constexpr int kQuery = MODE == 0 ? SA_TYPE_BF16 : MODE == 1 ? SA_TYPE_F16 : SA_TYPE_F32;
   extern __shared__ __align__(128) uint8_t kv4_smem[];
   __shared__ int scan_scratch[33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  uint8_t* ring = kv4_smem + warp * kStages * kEntry;
+  uint8_t* ring = kv4_smem + warp * Ring<NG>::kWarpBytes;
   int* starts = reinterpret_cast<int*>(kv4_smem + Ring<NG>::kBytes);
   const int lists = p.requests * p.lists_per_request;
 
   pdl_launch_dependents();
+  if (lane < kStages)
+    *reinterpret_cast<uint4*>(ring + lane * kStage + kEntry) = make_uint4(0u, 0u, 0u, 0u);
   // Entries before each list.
   int base = 0;
   for (int first = 0; first < lists; first += blockDim.x) {
@@ -273,20 +339,22 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i <= lists; i += blockDim.x) p.starts[i] = starts[i];
 
-  const int64_t entries = static_cast<int64_t>(base) * p.units_per_list;
-  const int64_t quota = quota_of(entries, static_cast<int64_t>(p.ctas) * kWarps);
-  // Neighbouring ranges go to different SMs: few entries still use them all.
-  const int64_t range = static_cast<int64_t>(warp) * p.ctas + blockIdx.x;
-  int64_t at = range * quota;
-  const int64_t end = min(at + quota, entries);
+  const Quota quota = quota_of(base * p.units_per_list, p.ctas);
+  const int cta_begin = min(static_cast<int>(blockIdx.x) * quota.cta, quota.entries);
+  const int cta_end = min(cta_begin + quota.cta, quota.entries);
+  const int warp_begin = min(cta_begin + warp * quota.warp, cta_end);
+  const int end = min(warp_begin + quota.warp, cta_end);
 
-  while (at < end) {
+  for (int at = warp_begin; at < end;) {
     // The unit of flat entry `at`, and the part of it in this warp's range.
-    const int list = list_of(starts, lists, static_cast<int>(at / p.units_per_list));
+    const int list = list_of(starts, lists, at / p.units_per_list);
     const int n = starts[list + 1] - starts[list];
-    const int64_t in_list = at - static_cast<int64_t>(starts[list]) * p.units_per_list;
-    const int unit = static_cast<int>(in_list / n), first = static_cast<int>(in_list % n);
-    const int count = static_cast<int>(min(static_cast<int64_t>(n - first), end - at));
+    const int in_list = at - starts[list] * p.units_per_list;
+    const int unit = in_list / n, first = in_list % n;
+    const int count = min(n - first, end - at);
+    // the CTA's whole range lies in this unit: its warps join their parts
+    const int unit_begin = at - first;
+    const bool joined = unit_begin <= cta_begin && unit_begin + n >= cta_end;
     const int b = list / p.lists_per_request;
     const int kv_head = list % p.lists_per_request * (p.kv_heads / p.lists_per_request) +
                         unit / p.row_tiles;
@@ -333,7 +401,7 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
           unread |= 1u << stage;
         } else {
           const uint8_t* from = head_pool + block * block_stride;
-          uint8_t* to = ring + stage * kEntry;
+          uint8_t* to = ring + stage * kStage;
 #pragma unroll
           for (int k = 0; k < (kPieces + 31) / 32; ++k) {
             // 32 NG pieces of keys, 32 NG of values in rows of 2 NG and 4 NG
@@ -358,8 +426,6 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
     float row_factor[NT][2];   // F of columns 2t, 2t + 1
     float row_sum[NT][NG][2];  // Q_g of columns 2t, 2t + 1
     int limit[NT][2];          // tokens that columns 2t, 2t + 1 see
-    bool row_live[NT][2];
-    int least = length;  // tokens that every row sees
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = row0 + nt * 8 + g;
@@ -371,10 +437,15 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
       float top = 0.0f;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
+        if (live) {
+          load16<kQuery>(p.query, from + 64 * gr, p.vector_rows, x[gr]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[gr][e] = 0.0f;
+        }
         sums[gr] = 0.0f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          x[gr][e] = live ? load_as_float(p.query, from + 64 * gr + e, p.query_type) : 0.0f;
           top = fmaxf(top, fabsf(x[gr][e]));
           sums[gr] += x[gr][e];
         }
@@ -414,17 +485,17 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         for (int gr = 0; gr < NG; ++gr)
           row_sum[nt][gr][c] = p.scale_log2 * __shfl_sync(0xffffffffu, sums[gr], source);
         const int r = row0 + nt * 8 + 2 * t + c;
-        row_live[nt][c] = r < p.rows;
-        limit[nt][c] = length - p.new_tokens + 1 + (row_live[nt][c] ? r / p.group : 0);
+        limit[nt][c] = length - p.new_tokens + 1 + (r < p.rows ? r / p.group : 0);
       }
     }
-    least = length - p.new_tokens + 1 + row0 / p.group;  // the tile's first row sees least
+    const int least = length - p.new_tokens + 1 + row0 / p.group;  // what every row sees
 
     float o[NT][NG][2][2][4];  // codes' sums of element 64 gr + 8 g + 4 w + 2 s (+ 1, times 16)
     float low[NT][2];          // minima's sums: lane group g holds value group g's
     float base[NT][2], sum[NT][2];  // running maximum - 11; sum of 2^(x - base)
     int step_log2 = 0;              // E: value steps are held as s * 2^-E
     uint32_t step_bits = 0;         // 2^E as FP16 bits, 0 before the first block
+    uint32_t step_unit = 0;         // 2^-E in both halves
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -546,12 +617,12 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         step[gr][1][1] = w.w;
       }
       {
-        const uint4 w = *reinterpret_cast<const uint4*>(entry + kv4_value_scales(kDim) + kDim +
-                                                        min(g, NG - 1) * 64 + t * 16);
-        minimum[0][0] = g < NG ? w.x : 0u;
-        minimum[0][1] = g < NG ? w.y : 0u;
-        minimum[1][0] = g < NG ? w.z : 0u;
-        minimum[1][1] = g < NG ? w.w : 0u;
+        const uint4 w = *reinterpret_cast<const uint4*>(
+            entry + (g < NG ? kv4_value_scales(kDim) + kDim + g * 64 + t * 16 : kEntry));
+        minimum[0][0] = w.x;
+        minimum[0][1] = w.y;
+        minimum[1][0] = w.z;
+        minimum[1][1] = w.w;
       }
       if constexpr (kMasked) {  // rows that are not held: nothing of them may enter a product
 #pragma unroll
@@ -570,9 +641,8 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
       uint32_t most = 0;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr)
-        most = hmax2(most, hmax2(hmax2(step[gr][0][0], step[gr][0][1]),
-                                 hmax2(step[gr][1][0], step[gr][1][1])));
-      most &= 0x7fff7fffu;
+        most = __vimax3_u16x2(__vimax3_u16x2(step[gr][0][0], step[gr][0][1], step[gr][1][0]),
+                              step[gr][1][1], most);
       bool passes = (most & 0xffffu) >= step_bits || most >> 16 >= step_bits;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -602,16 +672,18 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
                 o[nt][gr][k >> 1][k & 1][c + 2] *= keep;
               }
           }
-        most = hmax2(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = hmax2(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const uint32_t largest = max(most & 0xffffu, most >> 16);
+        uint32_t largest = max(most & 0xffffu, most >> 16);
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         if (largest >= step_bits) {  // the same in every lane
           // steps stay as they are while the largest is in [2^-8, 1)
           int exponent = static_cast<int>(largest >> 10) - 14;
           if (exponent > -8 && exponent <= 0) exponent = 0;
-          const float keep = step_bits == 0 ? 0.0f : exp2_approx(static_cast<float>(step_log2 - exponent));
+          const float keep = step_bits == 0 ? 0.0f : power_of_2(step_log2 - exponent);
           step_log2 = exponent;
           step_bits = static_cast<uint32_t>(exponent + 15) << 10;
+          const __half2 unit = __half2half2(__float2half_rn(power_of_2(-exponent)));
+          step_unit = *reinterpret_cast<const uint32_t*>(&unit);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -622,19 +694,6 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
                 for (int c = 0; c < 4; ++c) o[nt][gr][k >> 1][k & 1][c] *= keep;
         }
       }
-      uint32_t scaled_step[NG][2][2];
-      {
-        const __half2 unit = __half2half2(__float2half_rn(exp2_approx(static_cast<float>(-step_log2))));
-        const uint32_t unit_bits = *reinterpret_cast<const uint32_t*>(&unit);
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            scaled_step[gr][k >> 1][k & 1] = step_log2 == 0
-                                                 ? step[gr][k >> 1][k & 1]
-                                                 : hmul2(step[gr][k >> 1][k & 1], unit_bits);
-      }
-
       // ---- weights, as columns of the second product
       uint32_t weight[NT][kWeights][2][2];  // part, matrix step j, half h
 #pragma unroll
@@ -721,7 +780,7 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t s = scaled_step[gr][j][h];
+            const uint32_t s = hmul2(step[gr][j][h], step_unit);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               scaled[nt][0][j][h] = hmul2(weight[nt][0][j][h], s);
@@ -759,7 +818,7 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
       cp_async_wait<kStages - 1>();
       __syncwarp();
       if (!(unread >> stage & 1)) {
-        const uint8_t* entry = ring + stage * kEntry;
+        const uint8_t* entry = ring + stage * kStage;
         const int logical = ids ? newest : first + i;  // with ids, used for the newest block only
         const int token0 = logical * kBlockTokens;
         if ((!ids || first + i == n - 1) && token0 + kBlockTokens > least)
@@ -775,8 +834,10 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
 
     // ---- the segment's result
     const bool whole = count == n;
-    const int64_t part = range * 2 + (at == range * quota ? 0 : 1);
-    const float code_unit = exp2f(static_cast<float>((kCentred ? 0 : 24) + step_log2));
+    const int part = ((static_cast<int>(blockIdx.x) * kWarps + warp) * 2 + (at == warp_begin ? 0 : 1)) * kTile;
+    const float code_unit = power_of_2((kCentred ? 0 : 24) + step_log2);
+    const bool shared = joined && !whole;  // joined through shared memory
+    float* mine = reinterpret_cast<float*>(ring);  // [kTile][kDim], then [kTile][2]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -784,12 +845,9 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         float s = sum[nt][c];
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        const int r = nt * 8 + 2 * t + c;
+        const int r = nt * 8 + 2 * t + c, row = row0 + r;
         const float scale = whole ? (s != 0.0f ? 1.0f / s : 0.0f) : 1.0f;
-        const int row = row0 + r;
-        const int64_t out_row =
-            (static_cast<int64_t>(b) * p.new_tokens + row / p.group) * p.query_heads +
-            static_cast<int64_t>(kv_head) * p.group + row % p.group;
+        const int64_t out_row = output_row(p, b, kv_head, row);
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           const float minima = __shfl_sync(0xffffffffu, low[nt][c], gr * 4 + t);
@@ -800,83 +858,180 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
             y[2 * k] = fmaf(acc[c], code_unit, minima) * scale;
             y[2 * k + 1] = fmaf(acc[c + 2], code_unit * 0.0625f, minima) * scale;
           }
-          if (row_live[nt][c]) {
+          if (row < p.rows) {
+            const int e = 64 * gr + 8 * g;
             if (whole)
-              store8(p.out, out_row * kDim + 64 * gr + 8 * g, p.out_type, y);
+              store8(p.out, out_row * kDim + e, MODE == 2 ? p.out_type : kQuery, y);
+            else if (shared)
+              store8(mine, r * kDim + e, SA_TYPE_F32, y);
             else
-              store8(p.part_o, (part * kTile + r) * kDim + 64 * gr + 8 * g, SA_TYPE_F32, y);
+              store8(p.part_o, static_cast<int64_t>(part + r) * kDim + e, SA_TYPE_F32, y);
           }
         }
-        if (g == 0 && row_live[nt][c]) {
-          if (!whole) {
-            p.part_ml[(part * kTile + r) * 2] = base[nt][c];
-            p.part_ml[(part * kTile + r) * 2 + 1] = s;
-          } else if (p.lse) {
-            p.lse[out_row] =
-                s != 0.0f ? (base[nt][c] + log2f(s)) * 0.6931471805599453f : -INFINITY;
+        if (g == 0 && row < p.rows) {
+          if (whole) {
+            if (p.lse) p.lse[out_row] = log_of_sum(base[nt][c], s);
+          } else {
+            float* ml = shared ? mine + kTile * kDim + r * 2 : p.part_ml + (part + r) * 2;
+            ml[0] = base[nt][c];
+            ml[1] = s;
           }
         }
       }
+    if (shared) {
+      // Every active warp of the CTA has this one segment.
+      const int active = (cta_end - cta_begin + quota.warp - 1) / quota.warp;
+      if (active > 1)
+        asm volatile("bar.sync 1, %0;" ::"r"(active * 32) : "memory");
+      else
+        __syncwarp();
+      const bool complete = unit_begin == cta_begin && unit_begin + n == cta_end;
+      const int cta_part = static_cast<int>(blockIdx.x) * kWarps * 2 * kTile;
+      constexpr int kVectors = kDim / 4;
+      for (int i = threadIdx.x; i < kTile * kVectors; i += active * 32) {
+        const int r = i / kVectors, e = i % kVectors * 4, row = row0 + r;
+        if (row >= p.rows) break;
+        float top = -INFINITY, s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < active; ++w) {
+          const float* from = reinterpret_cast<const float*>(kv4_smem + w * Ring<NG>::kWarpBytes);
+          top = fmaxf(top, from[kTile * kDim + r * 2]);
+        }
+        for (int w = 0; w < active; ++w) {
+          const float* from = reinterpret_cast<const float*>(kv4_smem + w * Ring<NG>::kWarpBytes);
+          const float weight = exp2_approx(from[kTile * kDim + r * 2] - top);
+          s = fmaf(weight, from[kTile * kDim + r * 2 + 1], s);
+          const float4 v = *reinterpret_cast<const float4*>(from + r * kDim + e);
+          y[0] = fmaf(weight, v.x, y[0]);
+          y[1] = fmaf(weight, v.y, y[1]);
+          y[2] = fmaf(weight, v.z, y[2]);
+          y[3] = fmaf(weight, v.w, y[3]);
+        }
+        if (complete) {
+          const int64_t out_row = output_row(p, b, kv_head, row);
+          const float scale = s != 0.0f ? 1.0f / s : 0.0f;
+          store4(p.out, out_row * kDim + e, MODE == 2 ? p.out_type : kQuery, y[0] * scale,
+                 y[1] * scale, y[2] * scale, y[3] * scale);
+          if (p.lse && e == 0) p.lse[out_row] = log_of_sum(top, s);
+        } else {
+          store4(p.part_o, static_cast<int64_t>(cta_part + r) * kDim + e, SA_TYPE_F32, y[0], y[1],
+                 y[2], y[3]);
+          if (e == 0) {
+            p.part_ml[(cta_part + r) * 2] = top;
+            p.part_ml[(cta_part + r) * 2 + 1] = s;
+          }
+        }
+      }
+    }
     at += count;
   }
 }
 
 // Joins the parts of split units and writes the rows of empty ones: one CTA a
-// unit, a warp a query row.
+// query row, its warps sharing the parts.
 template <int NG>
-__global__ void __launch_bounds__(256) merge_kernel(const Kv4AttnParams p, int tile) {
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnParams p, int tile) {
   constexpr int kDim = 64 * NG, kPerLane = kDim / 32;
+  __shared__ float shared_o[kMergeWarps][kDim];
+  __shared__ float shared_ml[kMergeWarps][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int list = blockIdx.x / p.units_per_list, unit = blockIdx.x % p.units_per_list;
-  pdl_wait();
-  const int start = p.starts[list], n = p.starts[list + 1] - start;
-  const int64_t entries =
-      static_cast<int64_t>(p.starts[p.requests * p.lists_per_request]) * p.units_per_list;
-  const int64_t quota = quota_of(entries, static_cast<int64_t>(p.ctas) * kWarps);
-  const int64_t begin = static_cast<int64_t>(start) * p.units_per_list + static_cast<int64_t>(unit) * n;
-  const int64_t from = begin / quota, to = n ? (begin + n - 1) / quota : from;
-  if (n && from == to) return;  // written by its warp
+  const int rows = min(tile, p.rows);
+  const int r = blockIdx.x % rows, u = blockIdx.x / rows;
+  const int list = u / p.units_per_list, unit = u % p.units_per_list;
   const int b = list / p.lists_per_request;
   const int kv_head =
       list % p.lists_per_request * (p.kv_heads / p.lists_per_request) + unit / p.row_tiles;
-  const int row0 = unit % p.row_tiles * tile;
-  for (int r = warp; r < tile && row0 + r < p.rows; r += 8) {
-    float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
-    if (n) {
-      // The range of part k begins inside the unit, or (the first) before it.
-      auto slot = [&](int64_t k) { return (k * 2 + (k * quota >= begin ? 0 : 1)) * tile + r; };
-      for (int64_t k = from + lane; k <= to; k += 32) top = fmaxf(top, p.part_ml[slot(k) * 2]);
-#pragma unroll
-      for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-#pragma unroll 4
-      for (int64_t k = from; k <= to; ++k) {
-        const int64_t at = slot(k);
-        const float w = exp2_approx(p.part_ml[at * 2] - top);
-        sum = fmaf(w, p.part_ml[at * 2 + 1], sum);
-#pragma unroll
-        for (int j = 0; j < kPerLane; ++j)
-          o[j] = fmaf(w, p.part_o[at * kDim + j * 32 + lane], o[j]);
-      }
+  const int row = unit % p.row_tiles * tile + r;
+  pdl_wait();
+  if (row >= p.rows) return;
+  const int start = p.starts[list], n = p.starts[list + 1] - start;
+  const Quota quota =
+      quota_of(p.starts[p.requests * p.lists_per_request] * p.units_per_list, p.ctas);
+  const int begin = start * p.units_per_list + unit * n, end = begin + n;
+  // The unit's parts: those of the first CTA, one of each CTA between, those of
+  // the last; a CTA whose range lies in the unit has one.
+  int first = 0, parts = 0, first_parts = 0, last_warp = 0, first_warp = 0, ctas = 0;
+  if (n > 0) {
+    first = begin / quota.cta;
+    const int last = (end - 1) / quota.cta;
+    ctas = last - first + 1;
+    const auto covers = [&](int cta) {
+      return begin <= cta * quota.cta && end >= min((cta + 1) * quota.cta, quota.entries);
+    };
+    if (!covers(first)) first_warp = (begin - first * quota.cta) / quota.warp;
+    first_parts = covers(first) ? 1
+                                : (min(end - first * quota.cta, quota.cta) - 1) / quota.warp -
+                                      first_warp + 1;
+    parts = first_parts;
+    if (ctas > 1) {
+      last_warp = covers(last) ? 0 : (end - 1 - last * quota.cta) / quota.warp;
+      parts += ctas - 2 + last_warp + 1;
     }
-    const int row = row0 + r;
-    const int64_t out_row =
-        (static_cast<int64_t>(b) * p.new_tokens + row / p.group) * p.query_heads +
-        static_cast<int64_t>(kv_head) * p.group + row % p.group;
-    const float scale = sum != 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int j = 0; j < kPerLane; ++j) {
-      const int64_t e = out_row * kDim + j * 32 + lane;
-      const float y = o[j] * scale;
-      if (p.out_type == SA_TYPE_F32)
-        static_cast<float*>(p.out)[e] = y;
-      else if (p.out_type == SA_TYPE_F16)
-        static_cast<__half*>(p.out)[e] = __float2half_rn(y);
-      else
-        static_cast<__nv_bfloat16*>(p.out)[e] = __float2bfloat16_rn(y);
+    if (parts == 1) return;  // written by the attention
+  }
+  const auto slot = [&](int i) {  // row r of part i
+    int cta = first, w = first_warp + i;
+    if (i >= first_parts) {
+      i -= first_parts;
+      cta = first + 1 + min(i, ctas - 2);
+      w = max(i - (ctas - 2), 0);
     }
-    if (p.lse && lane == 0)
-      p.lse[out_row] =
-          sum != 0.0f ? (top + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    const bool inside = cta * quota.cta + w * quota.warp < begin;  // begins inside the warp's range
+    return ((cta * kWarps + w) * 2 + (inside ? 1 : 0)) * tile + r;
+  };
+  float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
+  for (int i = warp; i < parts; i += kMergeWarps * kMergeUnroll) {
+    float ml[kMergeUnroll][2], v[kMergeUnroll][kPerLane];
+#pragma unroll
+    for (int k = 0; k < kMergeUnroll; ++k) {
+      const int at = slot(min(i + k * kMergeWarps, parts - 1));
+      const float2 pair = *reinterpret_cast<const float2*>(p.part_ml + static_cast<int64_t>(at) * 2);
+      ml[k][0] = pair.x;
+      ml[k][1] = pair.y;
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j)
+        v[k][j] = p.part_o[static_cast<int64_t>(at) * kDim + j * 32 + lane];
+    }
+#pragma unroll
+    for (int k = 0; k < kMergeUnroll; ++k) {
+      if (i + k * kMergeWarps >= parts) break;
+      const float now = fmaxf(top, ml[k][0]);
+      const float keep = exp2_approx(top - now), weight = exp2_approx(ml[k][0] - now);
+      top = now;
+      sum = fmaf(sum, keep, weight * ml[k][1]);
+#pragma unroll
+      for (int j = 0; j < kPerLane; ++j) o[j] = fmaf(o[j], keep, weight * v[k][j]);
+    }
+  }
+  if (lane == 0) {
+    shared_ml[warp][0] = top;
+    shared_ml[warp][1] = sum;
+  }
+#pragma unroll
+  for (int j = 0; j < kPerLane; ++j) shared_o[warp][j * 32 + lane] = o[j];
+  __syncthreads();
+  top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, shared_ml[w][0]);
+  const int64_t out_row = output_row(p, b, kv_head, row);
+  for (int e = threadIdx.x; e < kDim; e += kMergeWarps * 32) {
+    float y = 0.0f;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+      if (w >= parts) break;
+      const float weight = exp2_approx(shared_ml[w][0] - top);
+      sum = fmaf(weight, shared_ml[w][1], sum);
+      y = fmaf(weight, shared_o[w][e], y);
+    }
+    y = sum != 0.0f ? y / sum : 0.0f;
+    const int64_t at = out_row * kDim + e;
+    if (p.out_type == SA_TYPE_F32)
+      static_cast<float*>(p.out)[at] = y;
+    else if (p.out_type == SA_TYPE_F16)
+      static_cast<__half*>(p.out)[at] = __float2half_rn(y);
+    else
+      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+    if (p.lse && e == 0) p.lse[out_row] = log_of_sum(top, sum);
   }
 }
 
@@ -903,8 +1058,9 @@ sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
   if (st != SA_OK) return st;
   const size_t smem = Ring<NG>::kBytes + (size_t)(lists + 1) * sizeof(int);
   SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(kWarps * 32), smem, stream, false, p));
-  return cuda_status(launch_kernel(merge_kernel<NG>, dim3(lists * p.units_per_list), dim3(256), 0,
-                                   stream, true, p, 8 * NT),
+  const int rows = std::min(p.rows, 8 * NT);
+  return cuda_status(launch_kernel(merge_kernel<NG>, dim3(lists * p.units_per_list * rows),
+                                   dim3(kMergeWarps * 32), 0, stream, true, p, 8 * NT),
                      "attention_kv4 merge launch");
 }
 
@@ -978,7 +1134,8 @@ extern "C" SA_API sa_status sa_attention_kv4(
   if (pool_blocks > kMost / kBlockTokens || table_blocks > kMost / kBlockTokens || budget >= kMost ||
       requests * lists * list_blocks > kMost)
     return fail(SA_ERR_UNSUPPORTED, "attention_kv4: more than 2^31 slots or listed blocks");
-  if (query_heads > kMost || new_tokens > kMost || requests * query_heads > kMost / new_tokens)
+  // every row of every tile, and every entry of every unit, has a 31-bit index
+  if (query_heads > 65536 || new_tokens > 65536 || requests * (query_heads + 16 * kv_heads) > kMost / new_tokens)
     return fail(SA_ERR_UNSUPPORTED, "attention_kv4: too many query rows");
   const size_t need =
       sa_attention_kv4_workspace_size(requests, new_tokens, query_heads, kv_heads, head_dim);
@@ -1013,7 +1170,12 @@ extern "C" SA_API sa_status sa_attention_kv4(
   const int tile = tile_rows((size_t)p.rows, head_dim, query_type);
   p.row_tiles = (p.rows + tile - 1) / tile;
   p.units_per_list = (int)(kv_heads / lists) * p.row_tiles;
+  if (requests * lists * list_blocks > (kMost >> 1) / (size_t)p.units_per_list)
+    return fail(SA_ERR_UNSUPPORTED, "attention_kv4: more than 2^30 (block, KV head, row tile) entries");
   p.scale_log2 = scale * 1.4426950408889634f;
+  const size_t element = query_type == SA_TYPE_F32 ? 4 : 2;
+  p.vector_rows = ((reinterpret_cast<uintptr_t>(query) | (size_t)stride_request * element |
+                    (size_t)stride_token * element | (size_t)stride_head * element) & 15u) == 0;
   p.ctas = max_warps(head_dim, tile) / kWarps;
   const size_t part_rows = (size_t)p.ctas * kWarps * 2 * tile;
   char* ws = static_cast<char*>(workspace);
