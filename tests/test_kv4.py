@@ -93,7 +93,7 @@ def _unpack_args(**over):
     (dict(value=None), "INVALID_ARG"), (dict(blocks=0), "INVALID_ARG"), (dict(heads=0), "INVALID_ARG"),
     (dict(type=3), "INVALID_ARG"), (dict(type=-1), "INVALID_ARG"), (dict(pool=8), "INVALID_ARG"),
     (dict(d=96), "UNSUPPORTED"), (dict(d=0), "UNSUPPORTED"), (dict(blocks=1 << 26), "UNSUPPORTED"),
-    (dict(tokens=1 << 31), "UNSUPPORTED"), (dict(tokens=1 << 30, heads=64), "UNSUPPORTED"),
+    (dict(tokens=1 << 31), "UNSUPPORTED"), (dict(heads=65537), "UNSUPPORTED"),
 ])
 def test_pack_and_unpack_refusals(pkg, over, status):
     lib = pkg.load()
