@@ -1,18 +1,23 @@
 // sa_kv4.cu -- rows into and out of the 4-bit cache.
 //
-// Both kernels move a row once and are bound by that traffic. A thread owns
-// eight consecutive elements (a column) of kTokens consecutive tokens: the
-// index arithmetic is done once, the tokens' loads are in flight together, and
-// the lanes of a warp read and write whole rows. Eight neighbouring lanes hold
-// a group of 64, so its minimum and maximum take three shuffles each.
+// Both kernels move a row once and are bound by that traffic. A thread owns 16
+// consecutive elements (a column) of kTokens consecutive tokens: the index
+// arithmetic is done once, the tokens' loads are in flight together, and the
+// lanes of a warp read and write whole rows. Four neighbouring lanes hold a
+// group of 64, so its minimum and maximum take two shuffles each. (Eight
+// elements of four tokens a thread spent 2.5 times the instructions: prompts of
+// 99,991 tokens, 5 heads of 64, packed and read back in 145 us.)
 //
 // Rounding. The step is the smallest FP16 number s with 15 s >= max - minimum
 // (the difference rounded up; 15 s is exact in FP32, so the comparison decides
-// as it would in exact arithmetic). A code is guessed as rint(x * (1 / s)) with
-// an approximate reciprocal and settled by its remainder x - code * s, which
-// is exact in FP32: only remainders of half a step or more, ties among them,
-// need a second look.
+// as it would in exact arithmetic). A code is rint(d / s) with d = x - minimum
+// in FP32: the reciprocal is held as the sum of two FP32 numbers, its error of
+// 2^-44 vanishes in the rounding of d * (r0 + r1) to FP32, so exact halves come
+// out exact and go to the even code; and no other quotient rounds to a half,
+// since d (24 bits) and a half times s (16 bits) that differ do so by more than
+// half a unit in the quotient's last place.
 #include <cfloat>
+#include <type_traits>
 
 #include "sa_kv4.cuh"
 
@@ -20,7 +25,7 @@ namespace sa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 4;  // consecutive tokens of a thread
+constexpr int kTokens = 2;  // consecutive tokens of a thread
 
 struct PackParams {
   uint8_t* pool;
@@ -31,7 +36,7 @@ struct PackParams {
   uint32_t* status;
   int64_t slot_limit;
   int tokens, kv_heads;
-  int columns;      // of 8 elements in a token's keys and values
+  int columns;      // of 16 elements in a token's keys and values
   int token_lanes;  // groups of kTokens tokens of a CTA
   int vectors;      // every row is 16-byte aligned
 };
@@ -46,31 +51,41 @@ struct UnpackParams {
   int tokens, kv_heads, columns, token_lanes;
 };
 
-// Eight elements of a row: `o`-th piece of group `group` of a head.
+// Sixteen elements of a row: the t-th part of group `group` of a head.
 struct Column {
-  int which, head, group, o;
+  int which, head, group, t;
   int64_t first;  // first token
   bool live;
 };
 template <int NG, class Params>
 __device__ __forceinline__ Column column_of(const Params& p) {
   Column c;
-  int lane = threadIdx.x, at = blockIdx.y * kThreads;
+  int lane = 0, at = blockIdx.y * kThreads + threadIdx.x;
   if (p.token_lanes > 1) {
     lane = threadIdx.x / p.columns;
     at = threadIdx.x % p.columns;
-  } else {
-    lane = 0;
-    at += threadIdx.x;
   }
   c.live = lane < p.token_lanes && at < p.columns;
   c.first = (static_cast<int64_t>(blockIdx.x) * p.token_lanes + lane) * kTokens;
-  c.o = at & 7;
-  c.group = (at >> 3) % NG;
-  const int rest = (at >> 3) / NG;
+  c.t = at & 3;
+  c.group = (at >> 2) % NG;
+  const int rest = (at >> 2) / NG;
   c.which = rest >= p.kv_heads ? 1 : 0;
   c.head = rest - (c.which ? p.kv_heads : 0);
   return c;
+}
+
+// The slots of a column's tokens, -1 where there is nothing to do.
+template <class Params>
+__device__ __forceinline__ void slots_of(const Params& p, const Column& c, int (&slot)[kTokens]) {
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    slot[i] = c.live && c.first + i < p.tokens ? p.slots[c.first + i] : -1;
+    if (slot[i] >= p.slot_limit) {
+      if (c.t == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
+      slot[i] = -1;
+    }
+  }
 }
 
 template <int NG>
@@ -78,90 +93,132 @@ __device__ __forceinline__ int64_t entry_of(int slot, int kv_heads, int head) {
   return (static_cast<int64_t>(slot / kBlockTokens) * kv_heads + head) * kv4_entry_bytes(64 * NG);
 }
 
-// Eight elements as FP32.
-template <int TYPE>
-__device__ __forceinline__ void load8(const void* base, int64_t at, bool vectors, float (&x)[8]) {
-  using Element = Kv4Type<TYPE>;
-  const auto* from = static_cast<const typename Element::T*>(base) + at;
-  if (vectors) {
-    if constexpr (TYPE == SA_TYPE_F32) {
-      const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-      x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-      const uint4 v = *reinterpret_cast<const uint4*>(from);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (TYPE == SA_TYPE_BF16) {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        } else {
-          const float2 f = h2x2f(w[i]);
-          x[2 * i] = f.x;
-          x[2 * i + 1] = f.y;
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Element::load(from[i]);
-  }
+// Minimum and maximum that are NaN if an operand is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float c;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+
+// Sixteen elements as they are loaded: 16-bit types stay packed until their
+// minimum and maximum are known.
+template <int TYPE>
+struct Row16 {
+  using Pair = std::conditional_t<TYPE == SA_TYPE_BF16, __nv_bfloat162, __half2>;
+  uint32_t word[8];
+  __device__ __forceinline__ void load(const void* base, int64_t at, bool vectors) {
+    const auto* from = static_cast<const uint16_t*>(base) + at;
+    if (vectors) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint4 v = reinterpret_cast<const uint4*>(from)[k];
+        word[4 * k] = v.x, word[4 * k + 1] = v.y, word[4 * k + 2] = v.z, word[4 * k + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) word[i] = from[2 * i] | static_cast<uint32_t>(from[2 * i + 1]) << 16;
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[i] = 0u;
+  }
+  __device__ __forceinline__ float value(int i) const {
+    const uint32_t w = word[i >> 1];
+    if constexpr (TYPE == SA_TYPE_BF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    return h2f(static_cast<uint16_t>(i & 1 ? w >> 16 : w));
+  }
+  __device__ __forceinline__ void limits(float& low, float& high) const {
+    Pair a = pair(0), b = a;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      a = __hmin2_nan(a, pair(i));
+      b = __hmax2_nan(b, pair(i));
+    }
+    low = min_nan(first(a), second(a));
+    high = max_nan(first(b), second(b));
+  }
+
+ private:
+  __device__ __forceinline__ Pair pair(int i) const { return *reinterpret_cast<const Pair*>(&word[i]); }
+  static __device__ __forceinline__ float first(Pair a) { return Kv4Type<TYPE>::load(a.x); }
+  static __device__ __forceinline__ float second(Pair a) { return Kv4Type<TYPE>::load(a.y); }
+};
+template <>
+struct Row16<SA_TYPE_F32> {
+  float x[16];
+  __device__ __forceinline__ void load(const void* base, int64_t at, bool vectors) {
+    const auto* from = static_cast<const float*>(base) + at;
+    if (vectors) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 v = reinterpret_cast<const float4*>(from)[k];
+        x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = from[i];
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+  }
+  __device__ __forceinline__ float value(int i) const { return x[i]; }
+  __device__ __forceinline__ void limits(float& low, float& high) const {
+    low = high = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) {
+      low = min_nan(low, x[i]);
+      high = max_nan(high, x[i]);
+    }
+  }
+};
 
 template <int TYPE, int NG>
 __global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams p) {
   constexpr int kDim = 64 * NG;
   const Column c = column_of<NG>(p);
-  float x[kTokens][8];
   int slot[kTokens];
-#pragma unroll
-  for (int i = 0; i < kTokens; ++i) {
-    slot[i] = c.live && c.first + i < p.tokens ? p.slots[c.first + i] : -1;
-    if (slot[i] >= p.slot_limit) {
-      if (c.o == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
-      slot[i] = -1;
-    }
-  }
+  slots_of(p, c, slot);
   const void* rows = c.which ? p.values : p.keys;
   const int64_t stride = c.which ? p.value_token_stride : p.key_token_stride;
   const int64_t at = c.first * stride +
                      c.head * (c.which ? p.value_head_stride : p.key_head_stride) +
-                     c.group * kKv4Group + c.o * 8;
+                     c.group * kKv4Group + c.t * 16;
+  Row16<TYPE> row[kTokens];
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
-    if (slot[i] >= 0) {
-      load8<TYPE>(rows, at + i * stride, p.vectors, x[i]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-    }
+    if (slot[i] >= 0)
+      row[i].load(rows, at + i * stride, p.vectors);
+    else
+      row[i].clear();
   }
-  uint32_t word[kTokens];
+  uint32_t word[kTokens][2];
   __half step[kTokens], minimum[kTokens];
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
-    float low = x[i][0], high = x[i][0];
-    bool nan = isnan(x[i][0]);
+    float low, high;
+    row[i].limits(low, high);
 #pragma unroll
-    for (int e = 1; e < 8; ++e) {
-      low = fminf(low, x[i][e]);
-      high = fmaxf(high, x[i][e]);
-      nan |= isnan(x[i][e]);
-    }
-    // NaN as an infinity, which no finite element gives
-    if (nan) high = INFINITY;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-      high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    for (int o = 1; o < 4; o <<= 1) {
+      low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
+      high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
     const bool finite = low >= -FLT_MAX && high <= FLT_MAX;
-    if constexpr (TYPE != SA_TYPE_F16) {
-      low = fmaxf(low, -65504.0f);
-      high = fminf(high, 65504.0f);
-      low = fminf(low, 65504.0f);
-      high = fmaxf(high, -65504.0f);
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = row[i].value(e);
+    if (TYPE != SA_TYPE_F16 && (low < -65504.0f || high > 65504.0f)) {
+      low = fminf(fmaxf(low, -65504.0f), 65504.0f);
+      high = fminf(fmaxf(high, -65504.0f), 65504.0f);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
     }
     minimum[i] = __float2half_rd(low);
     const float m = __half2float(minimum[i]), range = __fsub_ru(high, m);
@@ -171,37 +228,20 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams p) {
     for (int k = 0; k < 2; ++k)  // at most one FP16 number lies between them
       if (15.0f * h2f(bits) < range) ++bits;
     step[i] = __ushort_as_half(bits);
-    const float s = h2f(bits), inverse = s > 0.0f ? __fdividef(1.0f, s) : 0.0f;
+    const float s = h2f(bits), r0 = s > 0.0f ? __fdividef(1.0f, s) : 0.0f;
+    const float r1 = fmaf(-s, r0, 1.0f) * r0;
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer
-    uint32_t sum = 0;
-    float most = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float y = x[i][e];
-      if constexpr (TYPE != SA_TYPE_F16) y = fminf(fmaxf(y, -65504.0f), 65504.0f);
-      x[i][e] = y - m;
-      const float rounded = fmaf(x[i][e], inverse, kMagic);
-      sum += __float_as_uint(rounded) << (4 * e);
-      most = fmaxf(most, fabsf(fmaf(-(rounded - kMagic), s, x[i][e])));
-    }
-    sum -= 0x11111111u * 0x4b400000u;  // kMagic's bits, eight times
-    if (2.0f * most >= s) {
-      sum = 0;
+    for (int k = 0; k < 2; ++k) {
+      uint32_t sum = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float code = fmaf(x[i][e], inverse, kMagic) - kMagic;
-        const float twice = 2.0f * fmaf(-code, s, x[i][e]);
-        const bool odd = static_cast<int>(code) & 1;
-        if (twice > s || (twice == s && odd)) code += 1.0f;
-        if (twice < -s || (twice == -s && odd)) code -= 1.0f;
-        sum |= static_cast<uint32_t>(s > 0.0f ? code : 0.0f) << (4 * e);
+        const float d = x[8 * k + e] - m;
+        sum += __float_as_uint(fmaf(d, r0, d * r1) + kMagic) << (4 * e);
       }
+      word[i][k] = finite ? sum - 0x11111111u * 0x4b400000u : 0u;  // without kMagic's bits
     }
-    word[i] = sum;
-    if (!finite) {
-      word[i] = 0;
-      step[i] = minimum[i] = __ushort_as_half(0x7fffu);
-    }
+    if (!finite) step[i] = minimum[i] = __ushort_as_half(0x7fffu);
   }
   if (c.which == 0) {
 #pragma unroll
@@ -209,31 +249,36 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams p) {
       if (slot[i] < 0) continue;
       const int r = slot[i] % kBlockTokens;
       uint8_t* entry = p.pool + entry_of<NG>(slot[i], p.kv_heads, c.head);
-      *reinterpret_cast<uint32_t*>(entry + kv4_key_at(kDim, r, c.group, c.o >> 1) +
-                                   4 * (c.o & 1)) = word[i];
-      if (c.o == 0)
+      *reinterpret_cast<uint2*>(entry + kv4_key_at(kDim, r, c.group, c.t)) =
+          make_uint2(word[i][0], word[i][1]);
+      if (c.t == 0)
         *reinterpret_cast<__half2*>(entry + kv4_key_scale_at(kDim, r, c.group)) =
             __halves2half2(step[i], minimum[i]);
     }
   } else {
+    // the two tokens of a pair row at once where the slots allow it
+    const bool pair = slot[0] >= 0 && (slot[0] & 1) == 0 && slot[1] == slot[0] + 1;
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
       if (slot[i] < 0) continue;
       const int r = slot[i] % kBlockTokens;
       uint8_t* entry = p.pool + entry_of<NG>(slot[i], p.kv_heads, c.head);
-      if (c.o == 0) {
-        __half* at = reinterpret_cast<__half*>(entry + kv4_value_scale_at(kDim, r, c.group));
-        at[0] = step[i];
-        at[kDim / 2] = minimum[i];
+      if (c.t == 0) {
+        __half* to = reinterpret_cast<__half*>(entry + kv4_value_scale_at(kDim, r, c.group));
+        to[0] = step[i];
+        to[kDim / 2] = minimum[i];
       }
-      uint8_t* to = entry + kv4_value_at(kDim, r, c.group, c.o, 0, 0);
-      // two tokens of a pair row at once, or the 16-bit pieces of one
-      if (i + 1 < kTokens && (r & 1) == 0 && slot[i + 1 < kTokens ? i + 1 : i] == slot[i] + 1) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(__byte_perm(word[i], word[i + 1 < kTokens ? i + 1 : i], 0x5410),
-                                                   __byte_perm(word[i], word[i + 1 < kTokens ? i + 1 : i], 0x7632));
-      } else if (!(i > 0 && (r & 1) == 1 && slot[i > 0 ? i - 1 : i] == slot[i] - 1)) {
-        *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(word[i]);
-        *reinterpret_cast<uint16_t*>(to + 4) = static_cast<uint16_t>(word[i] >> 16);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        uint8_t* to = entry + kv4_value_at(kDim, r, c.group, 2 * c.t + k, 0, 0);
+        if (pair) {
+          if (i == 0)
+            *reinterpret_cast<uint2*>(to) = make_uint2(__byte_perm(word[0][k], word[1][k], 0x5410),
+                                                       __byte_perm(word[0][k], word[1][k], 0x7632));
+        } else {
+          *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(word[i][k]);
+          *reinterpret_cast<uint16_t*>(to + 4) = static_cast<uint16_t>(word[i][k] >> 16);
+        }
       }
     }
   }
@@ -246,34 +291,31 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const UnpackParams p) 
   const Column c = column_of<NG>(p);
   if (!c.live) return;
   int slot[kTokens];
-#pragma unroll
-  for (int i = 0; i < kTokens; ++i) {
-    slot[i] = c.first + i < p.tokens ? p.slots[c.first + i] : -1;
-    if (slot[i] >= p.slot_limit) {
-      if (c.o == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
-      slot[i] = -1;
-    }
-  }
-  uint32_t word[kTokens];
+  slots_of(p, c, slot);
+  uint32_t word[kTokens][2];
   __half step[kTokens], minimum[kTokens];
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
-    word[i] = 0;
+    word[i][0] = word[i][1] = 0;
     step[i] = minimum[i] = __ushort_as_half(0);
     if (slot[i] < 0) continue;
     const int r = slot[i] % kBlockTokens;
     const uint8_t* entry = p.pool + entry_of<NG>(slot[i], p.kv_heads, c.head);
     if (c.which == 0) {
-      word[i] = *reinterpret_cast<const uint32_t*>(
-          entry + kv4_key_at(kDim, r, c.group, c.o >> 1) + 4 * (c.o & 1));
+      const uint2 w = *reinterpret_cast<const uint2*>(entry + kv4_key_at(kDim, r, c.group, c.t));
+      word[i][0] = w.x;
+      word[i][1] = w.y;
       const __half2 sm =
           *reinterpret_cast<const __half2*>(entry + kv4_key_scale_at(kDim, r, c.group));
       step[i] = __low2half(sm);
       minimum[i] = __high2half(sm);
     } else {
-      const uint2 pair =
-          *reinterpret_cast<const uint2*>(entry + kv4_value_at(kDim, r & ~1, c.group, c.o, 0, 0));
-      word[i] = __byte_perm(pair.x, pair.y, r & 1 ? 0x7632 : 0x5410);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint2 w = *reinterpret_cast<const uint2*>(
+            entry + kv4_value_at(kDim, r & ~1, c.group, 2 * c.t + k, 0, 0));
+        word[i][k] = __byte_perm(w.x, w.y, r & 1 ? 0x7632 : 0x5410);
+      }
       const __half* at =
           reinterpret_cast<const __half*>(entry + kv4_value_scale_at(kDim, r, c.group));
       step[i] = at[0];
@@ -281,15 +323,23 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const UnpackParams p) 
     }
   }
   auto* row = static_cast<typename Element::T*>(c.which ? p.values : p.keys) +
-              (c.first * p.kv_heads + c.head) * kDim + c.group * kKv4Group + c.o * 8;
+              (c.first * p.kv_heads + c.head) * kDim + c.group * kKv4Group + c.t * 16;
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
     if (c.first + i >= p.tokens) break;
     const float s = __half2float(step[i]), m = __half2float(minimum[i]);
-    alignas(16) typename Element::T y[8];
+    alignas(16) typename Element::T y[16];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)  // the product is exact, so this rounds once
-      y[e] = Element::store(fmaf(s, static_cast<float>((word[i] >> (4 * e)) & 15u), m));
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // codes e and e + 4 as 1024 + c, then c, in FP16
+        const uint32_t both = (word[i][k] >> (4 * e) & 0x000f000fu) | 0x64006400u;
+        const float2 code = __half22float2(
+            __hsub2(*reinterpret_cast<const __half2*>(&both), __half2half2(__ushort_as_half(0x6400u))));
+        y[8 * k + e] = Element::store(fmaf(s, code.x, m));  // the product is exact: one rounding
+        y[8 * k + e + 4] = Element::store(fmaf(s, code.y, m));
+      }
 #pragma unroll
     for (int k = 0; k < static_cast<int>(sizeof(y) / 16); ++k)
       reinterpret_cast<uint4*>(row + static_cast<int64_t>(i) * p.kv_heads * kDim)[k] =
@@ -325,7 +375,7 @@ template <class Params>
 dim3 row_grid(Params& p, size_t tokens, size_t kv_heads, size_t head_dim) {
   p.tokens = (int)tokens;
   p.kv_heads = (int)kv_heads;
-  p.columns = (int)(2 * kv_heads * (head_dim / 8));
+  p.columns = (int)(2 * kv_heads * (head_dim / 16));
   p.token_lanes = p.columns < kThreads ? kThreads / p.columns : 1;
   const size_t each = (size_t)p.token_lanes * kTokens;
   return dim3((unsigned)((tokens + each - 1) / each), (unsigned)((p.columns + kThreads - 1) / kThreads));
