@@ -289,7 +289,6 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const UnpackParams p) 
   using Element = Kv4Type<TYPE>;
   constexpr int kDim = 64 * NG;
   const Column c = column_of<NG>(p);
-  if (!c.live) return;
   int slot[kTokens];
   slots_of(p, c, slot);
   uint32_t word[kTokens][2];
@@ -326,7 +325,6 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const UnpackParams p) 
               (c.first * p.kv_heads + c.head) * kDim + c.group * kKv4Group + c.t * 16;
 #pragma unroll
   for (int i = 0; i < kTokens; ++i) {
-    if (c.first + i >= p.tokens) break;
     const float s = __half2float(step[i]), m = __half2float(minimum[i]);
     alignas(16) typename Element::T y[16];
 #pragma unroll
@@ -340,10 +338,25 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const UnpackParams p) 
         y[8 * k + e] = Element::store(fmaf(s, code.x, m));  // the product is exact: one rounding
         y[8 * k + e + 4] = Element::store(fmaf(s, code.y, m));
       }
+    // Two lanes exchange quads, so that each store of the warp writes whole
+    // 32-byte sectors.
+    uint4* to = reinterpret_cast<uint4*>(row + static_cast<int64_t>(i) * p.kv_heads * kDim);
+    const uint4* from = reinterpret_cast<const uint4*>(y);
+    constexpr int kQuads = static_cast<int>(sizeof(y) / 16);
+    const bool odd = threadIdx.x & 1, writes = c.live && c.first + i < p.tokens;
 #pragma unroll
-    for (int k = 0; k < static_cast<int>(sizeof(y) / 16); ++k)
-      reinterpret_cast<uint4*>(row + static_cast<int64_t>(i) * p.kv_heads * kDim)[k] =
-          reinterpret_cast<const uint4*>(y)[k];
+    for (int k = 0; k < kQuads; k += 2) {
+      const uint4 keep = odd ? from[k + 1] : from[k], give = odd ? from[k] : from[k + 1];
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, give.x, 1);
+      got.y = __shfl_xor_sync(0xffffffffu, give.y, 1);
+      got.z = __shfl_xor_sync(0xffffffffu, give.z, 1);
+      got.w = __shfl_xor_sync(0xffffffffu, give.w, 1);
+      if (writes) {
+        to[odd ? k + 1 - kQuads : k] = odd ? got : keep;  // the even lane's quads
+        to[odd ? k + 1 : k + kQuads] = odd ? keep : got;  // the odd lane's
+      }
+    }
   }
 }
 
