@@ -17,6 +17,7 @@ the kernels raise; the formats and rules stand in include/sa_b200.h.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -56,13 +57,24 @@ def _status(status, device):
     return None if status is None else _tensor(status, torch.int32, 1, "status", device)
 
 
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The current stream's handle without a Stream object around it (0.1 us, not 2.2).
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
+
+
 def _call(device, what, fn, *args) -> None:
-    """fn(*args, stream) with the current stream of `device`."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    """fn(*args, stream) with the current stream of `device`, made current for the call."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, _stream_of(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+            status = fn(*args, _stream_of(index))
+    if status:
+        check(status, what)
 
 
 def _pool_dims(pool) -> tuple[int, int, int, int]:
@@ -108,8 +120,7 @@ def plan_blocks(add: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Te
         raise ValueError("add, seq_lens and block_table must have a row a request, free_top one element")
     if max_tokens < 0:
         raise ValueError("max_tokens must not be negative")
-    out = torch.empty(2 * max_tokens + n + 1, dtype=torch.int32, device=dev)
-    slots, positions, cu = out.split([max_tokens, max_tokens, n + 1])
+    slots, positions, cu = add.new_empty(max_tokens), add.new_empty(max_tokens), add.new_empty(n + 1)
     _call(dev, "plan_blocks", load().sa_plan_blocks, ptr, n, lens, table, block_table.shape[1], free,
           free_list.shape[0], top, max_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
           _status(status, dev))
@@ -145,10 +156,16 @@ def unpack_kv4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = tor
         raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     tokens = slots.shape[0]
     key = torch.empty(tokens, heads, d, dtype=dtype, device=dev)
-    value = torch.empty_like(key)
+    value = key.new_empty(key.shape)
     _call(dev, "unpack_kv4", load().sa_unpack_kv4, ptr, blocks, at, tokens, heads, d, key.data_ptr(),
           value.data_ptr(), _TYPES[dtype], _status(status, dev))
     return key, value
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(n, new, qh, heads, d, index) -> int:
+    with torch.cuda.device(index):
+        return load().sa_attention_kv4_workspace_size(n, new, qh, heads, d)
 
 
 def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Tensor,
@@ -195,12 +212,12 @@ def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Te
     out_dtype = query.dtype if out_dtype is None else out_dtype
     if out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    out = torch.empty(query.shape, dtype=out_dtype, device=dev)
+    out = query.new_empty(query.shape, dtype=out_dtype)
     lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    ws_bytes = lib.sa_attention_kv4_workspace_size(n, new, qh, heads, d)
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+    ws_bytes = _workspace_bytes(n, new, qh, heads, d, dev.index)
+    ws = pool.new_empty(ws_bytes or 16)
     _call(dev, "attention_kv4", lib.sa_attention_kv4, q, _TYPES[query.dtype], query.stride(0),
           query.stride(1) if lead == 4 else 0, query.stride(-2), ptr, blocks, table,
           block_table.shape[1], lens, ids, counts, groups, budget, n, new, qh, heads, d, scale,
