@@ -319,25 +319,45 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
   int* starts = reinterpret_cast<int*>(kv4_smem + Ring<NG>::kBytes);
   const int lists = p.requests * p.lists_per_request;
 
-  pdl_launch_dependents();
   if (lane < kStages)
     *reinterpret_cast<uint4*>(ring + lane * kStage + kEntry) = make_uint4(0u, 0u, 0u, 0u);
-  // Entries before each list.
+  // Entries before each list. Up to 32 lists each warp sums by itself (all
+  // write the same values) and needs no barrier.
   int base = 0;
-  for (int first = 0; first < lists; first += blockDim.x) {
-    const int list = first + threadIdx.x;
+  if (lists <= 32) {
     bool bad = false;
-    const int n = list < lists ? list_entries(p, list, &bad) : 0;
-    if (bad && blockIdx.x == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
-    int total;
-    const int before = base + block_exclusive_scan(n, scan_scratch, &total);
-    if (list < lists) starts[list] = before;
-    base += total;
+    const int n = lane < lists ? list_entries(p, lane, &bad) : 0;
+    if (bad && blockIdx.x == 0 && warp == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
+    int inclusive = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, inclusive, o);
+      if (lane >= o) inclusive += before;
+    }
+    base = __shfl_sync(0xffffffffu, inclusive, 31);
+    if (lane < lists) starts[lane + 1] = inclusive;
+    if (lane == 0) starts[0] = 0;
+    if (blockIdx.x == 0 && warp == 0) {
+      if (lane < lists) p.starts[lane + 1] = inclusive;
+      if (lane == 0) p.starts[0] = 0;
+    }
+    __syncwarp();
+  } else {
+    for (int first = 0; first < lists; first += blockDim.x) {
+      const int list = first + threadIdx.x;
+      bool bad = false;
+      const int n = list < lists ? list_entries(p, list, &bad) : 0;
+      if (bad && blockIdx.x == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
+      int total;
+      const int before = base + block_exclusive_scan(n, scan_scratch, &total);
+      if (list < lists) starts[list] = before;
+      base += total;
+    }
+    if (threadIdx.x == 0) starts[lists] = base;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= lists; i += blockDim.x) p.starts[i] = starts[i];
   }
-  if (threadIdx.x == 0) starts[lists] = base;
-  __syncthreads();
-  if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i <= lists; i += blockDim.x) p.starts[i] = starts[i];
 
   const Quota quota = quota_of(base * p.units_per_list, p.ctas);
   const int cta_begin = min(static_cast<int>(blockIdx.x) * quota.cta, quota.entries);
@@ -941,7 +961,6 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
   const int kv_head =
       list % p.lists_per_request * (p.kv_heads / p.lists_per_request) + unit / p.row_tiles;
   const int row = unit % p.row_tiles * tile + r;
-  pdl_wait();
   if (row >= p.rows) return;
   const int start = p.starts[list], n = p.starts[list + 1] - start;
   const Quota quota =
@@ -1060,7 +1079,7 @@ sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
   SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(kWarps * 32), smem, stream, false, p));
   const int rows = std::min(p.rows, 8 * NT);
   return cuda_status(launch_kernel(merge_kernel<NG>, dim3(lists * p.units_per_list * rows),
-                                   dim3(kMergeWarps * 32), 0, stream, true, p, 8 * NT),
+                                   dim3(kMergeWarps * 32), 0, stream, false, p, 8 * NT),
                      "attention_kv4 merge launch");
 }
 
