@@ -122,6 +122,12 @@ __device__ __forceinline__ void store4(void* base, int64_t i, int type, float a,
         make_uint2(pack_bf162(a, b), pack_bf162(c, d));
 }
 
+__device__ __forceinline__ void cp_async16_at(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to),
+               "l"(reinterpret_cast<uint64_t>(from))
+               : "memory");
+}
+
 // ---- matrix fragments -------------------------------------------------------------
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -318,6 +324,12 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
   uint8_t* ring = kv4_smem + warp * Ring<NG>::kWarpBytes;
   int* starts = reinterpret_cast<int*>(kv4_smem + Ring<NG>::kBytes);
   const int lists = p.requests * p.lists_per_request;
+  // Where a lane's 16-byte pieces of an entry go: piece 32 k + lane of the keys
+  // and of the values (k even, odd), less 512 k bytes.
+  const uint32_t ring_at = smem_addr(ring);
+  const uint32_t key_place = 16 * (lane ^ key_swizzle<NG>(lane / (2 * NG)));
+  const uint32_t value_place[2] = {16u * (lane ^ value_swizzle<NG>(lane / (4 * NG))),
+                                   16u * (lane ^ value_swizzle<NG>((32 + lane) / (4 * NG)))};
 
   if (lane < kStages)
     *reinterpret_cast<uint4*>(ring + lane * kStage + kEntry) = make_uint4(0u, 0u, 0u, 0u);
@@ -384,7 +396,7 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_blocks;
     const int32_t* ids =
         p.selected ? p.selected + static_cast<int64_t>(list) * p.budget : nullptr;
-    const uint8_t* head_pool = p.pool + static_cast<int64_t>(kv_head) * kEntry;
+    const uint8_t* lane_pool = p.pool + static_cast<int64_t>(kv_head) * kEntry + 16 * lane;
     const int64_t block_stride = static_cast<int64_t>(p.kv_heads) * kEntry;
 
     // Physical blocks of 32 entries from `from` on, one per lane; -1 where
@@ -420,19 +432,15 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         if (block < 0) {
           unread |= 1u << stage;
         } else {
-          const uint8_t* from = head_pool + block * block_stride;
-          uint8_t* to = ring + stage * kStage;
+          // 32 NG pieces of keys, 32 NG of values in rows of 2 NG and 4 NG
+          // pieces, then the scales
+          const uint8_t* from = lane_pool + block * block_stride;
+          const uint32_t to = ring_at + stage * kStage;
 #pragma unroll
           for (int k = 0; k < (kPieces + 31) / 32; ++k) {
-            // 32 NG pieces of keys, 32 NG of values in rows of 2 NG and 4 NG
-            // pieces, then the scales
-            const int piece = k * 32 + lane;
-            int place = piece;
-            if (k < 2 * NG)
-              place ^= key_swizzle<NG>(piece / (2 * NG));
-            else if (k < 4 * NG)
-              place ^= value_swizzle<NG>((piece - 64 * NG) / (4 * NG));
-            if (kPieces % 32 == 0 || piece < kPieces) cp_async16(to + place * 16, from + piece * 16);
+            const uint32_t place = k < 2 * NG ? key_place : k < 4 * NG ? value_place[k & 1] : 16 * lane;
+            if (kPieces % 32 == 0 || k * 32 + lane < kPieces)
+              cp_async16_at(to + place + 512 * k, from + 512 * k);
           }
         }
       }
