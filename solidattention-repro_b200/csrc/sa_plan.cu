@@ -16,16 +16,19 @@
 //
 // The work is a few bytes a request and 8 a token, and its time is the chain
 // of dependent reads (lengths, scan, list, table), so it is one launch: a
-// single CTA for small steps, one cluster of 8 for large ones (the scans are
-// repeated in each CTA, the writes are split; a cluster barrier orders the
-// blocks taken before the table is read).
+// single CTA for small steps, one cluster for large ones (the scans are
+// repeated in each CTA, the writes are split; a cluster barrier stands between
+// the last read of the old state and the first write over it).
 #include "sa_device.cuh"
 
 namespace sa {
 namespace {
 
 constexpr int kPlanMaxRequests = 8192;
-constexpr int kPlanCluster = 8;
+constexpr int kPlanArrays = 5;  // of one int a request in shared memory
+constexpr int kFew = 4;         // new tokens that a request's own thread writes
+constexpr int kChunk = 128;     // new tokens that a warp writes at a time otherwise
+constexpr int kPlanCluster = 16;  // the largest; 8 took 21 us for 2,000 requests with 156,200 tokens
 
 struct PlanParams {
   const int32_t* add;
@@ -52,32 +55,41 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Exclusive sum over the block's threads; *total gets the block's sum.
-__device__ __forceinline__ long long scan64(long long value, long long* scratch,
-                                            long long* total) {
+// Exclusive sums of N values over the block's threads; totals get the block's.
+// narrow: over each warp's lanes alone (the warps hold the same values).
+template <int N>
+__device__ __forceinline__ void scan64(const long long (&value)[N], long long (&before)[N],
+                                       long long (&totals)[N], long long (*scratch)[32],
+                                       bool narrow) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  long long inclusive = value;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long n = __shfl_up_sync(0xffffffffu, inclusive, o);
-    if (lane >= o) inclusive += n;
-  }
-  if (lane == 31) scratch[warp] = inclusive;
-  __syncthreads();
-  if (warp == 0) {
-    long long w = lane < warps ? scratch[lane] : 0;
+  for (int i = 0; i < N; ++i) {
+    long long sum = value[i];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long n = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += n;
+      const long long n = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += n;
     }
-    scratch[lane] = w;
+    before[i] = sum - value[i];
+    totals[i] = __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (narrow) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (lane == 0) scratch[i][warp] = totals[i];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {  // every warp sums the warps' totals for itself
+    const long long mine = lane < warps ? scratch[i][lane] : 0;
+    long long sum = mine;
+    for (int o = 1; o < warps; o <<= 1) {
+      const long long n = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += n;
+    }
+    totals[i] = __shfl_sync(0xffffffffu, sum, warps - 1);
+    before[i] += __shfl_sync(0xffffffffu, sum - mine, warp);
   }
   __syncthreads();
-  const long long before = (warp > 0 ? scratch[warp - 1] : 0) + inclusive - value;
-  *total = scratch[warps - 1];
-  __syncthreads();
-  return before;
 }
 
 // The last index in [0, n) whose start is not above `at` (starts[0] is 0).
@@ -97,15 +109,38 @@ __device__ __forceinline__ int blocks_of(int tokens) {
   return static_cast<int>((static_cast<long long>(tokens) + kBlockTokens - 1) / kBlockTokens);
 }
 
+// Slot and position of a request's k-th new token, row i: its block is in the
+// table if the request held it, else in the list. `len`: the length before, bit
+// 31 set when the request is refused; `take`: its first block in taking order.
+__device__ __forceinline__ void write_token(const PlanParams& p, int i, int k, int len, int take,
+                                            int b, int top) {
+  const int before = len & 0x7fffffff;
+  const int position =
+      static_cast<int>(min(static_cast<long long>(before) + k, 0x7fffffffll));  // far only when refused
+  int slot = -1;
+  if (len >= 0) {
+    const int at = position / kBlockTokens, held = blocks_of(before);
+    const int block = at < held ? p.table[static_cast<int64_t>(b) * p.table_blocks + at]
+                                : p.free_list[top - 1 - (take + at - held)];
+    if (block >= 0 && block < p.pool_blocks)
+      slot = block * kBlockTokens + position % kBlockTokens;
+    else
+      raise_status(p.status, SA_DEV_BAD_BLOCK);
+  }
+  p.slots[i] = slot;
+  if (p.positions) p.positions[i] = position;
+}
+
 __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
   extern __shared__ int32_t plan_smem[];
-  __shared__ long long scratch[32];
+  __shared__ long long scratch[3][32];
   __shared__ int taken_shared;
   const int n = p.requests, rank = blockIdx.x, ctas = cluster_ctas();
   int32_t* tok = plan_smem;       // [n] first row of a request's new tokens
   int32_t* take = tok + n;        // [n] first of its blocks in taking order
   int32_t* give = take + n;       // [n] first of its blocks in giving order
   int32_t* len = give + n;        // [n] its length before, bit 31 set when refused
+  int32_t* chunk = len + n;       // [n] first of its chunks of kChunk tokens
   if (threadIdx.x == 0) taken_shared = 0;
 
   int top = *p.free_top;
@@ -113,38 +148,53 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
     if (rank == 0 && threadIdx.x == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
     top = min(max(top, 0), p.pool_blocks);
   }
-  long long tok_base = 0, take_base = 0, give_base = 0;
+  long long tok_base = 0, take_base = 0, give_base = 0, chunk_base = 0;
   const long long limit = static_cast<long long>(p.table_blocks) * kBlockTokens;
+  const bool narrow = n <= 32;  // every warp scans all requests itself
   for (int first = 0; first < n; first += blockDim.x) {
-    const int b = first + threadIdx.x;
+    const int b = narrow ? threadIdx.x & 31 : first + threadIdx.x;
     const bool live = b < n;
     const int before = live ? p.seq_lens[b] : 0;
     const int add = live ? p.add[b] : 0;
     const bool broken = before < 0 || before > limit;
     const long long after = broken ? 0 : max(0ll, static_cast<long long>(before) + add);
     const long long grow = max(add, 0);
-    long long total;
-    const long long tok_at = tok_base + scan64(grow, scratch, &total);
-    tok_base += total;
+    long long grown[1] = {grow}, grown_before[1], grown_total[1];
+    scan64(grown, grown_before, grown_total, scratch, narrow);
+    const long long tok_at = tok_base + grown_before[0];
+    tok_base += grown_total[0];
     const bool full = !broken && after > limit;
     const bool over = tok_at + grow > p.max_tokens;
     bool refused = broken || full || over;
     const int held = broken ? 0 : blocks_of(before);
     const int want = refused ? held : blocks_of(static_cast<int>(after));
     const int need = max(want - held, 0);
-    const long long take_at = take_base + scan64(need, scratch, &total);
-    take_base += total;
+    // blocks taken and given back (a request that gives back is not refused below)
+    const bool few = grow <= kFew;
+    // rows inside the slot map: row indices stay below max_tokens + kChunk
+    const long long rows = min(grow, max(p.max_tokens - tok_at, 0ll));
+    long long moved[3] = {need, max(held - want, 0), few ? 0 : (rows + kChunk - 1) / kChunk};
+    long long moved_before[3], moved_total[3];
+    scan64(moved, moved_before, moved_total, scratch, narrow);
+    const long long take_at = take_base + moved_before[0], give_at = give_base + moved_before[1];
+    take_base += moved_total[0];
+    give_base += moved_total[1];
+    const long long chunk_at = chunk_base + moved_before[2];
+    chunk_base += moved_total[2];
     const bool short_of = need > 0 && take_at + need > top;
     refused |= short_of;
     if (need > 0 && !short_of) atomicMax(&taken_shared, static_cast<int>(take_at + need));
-    const long long give_at = give_base + scan64(max(held - want, 0), scratch, &total);
-    give_base += total;
     if (live) {
       tok[b] = static_cast<int>(min(tok_at, 0x7fffffffll));
       take[b] = static_cast<int>(min(take_at, 0x7fffffffll));
       give[b] = static_cast<int>(give_at);
       len[b] = (broken ? 0 : before) | (refused ? static_cast<int>(0x80000000u) : 0);
-      if (rank == 0) {
+      chunk[b] = static_cast<int>(chunk_at);
+      // requests that grow by a few tokens write them at once, those of 32 in one CTA
+      if (few && (b >> 5) % ctas == rank && (!narrow || threadIdx.x < 32))
+        for (int k = 0; k < rows; ++k)
+          write_token(p, tok[b] + k, k, len[b], take[b], b, top);
+      if (rank == 0 && (!narrow || threadIdx.x < 32)) {
         if (broken) raise_status(p.status, SA_DEV_BAD_BLOCK);
         if (full) raise_status(p.status, SA_DEV_TABLE_FULL);
         if (over && !broken && !full) raise_status(p.status, SA_DEV_SLOTS_FULL);
@@ -156,6 +206,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
   const int taken = taken_shared;
   const int given = static_cast<int>(min(give_base, static_cast<long long>(0x7fffffff)));
   const int tokens = static_cast<int>(min(tok_base, static_cast<long long>(p.max_tokens)));
+  const int chunks = static_cast<int>(chunk_base);
   const int me = rank * blockDim.x + threadIdx.x, all = ctas * blockDim.x;
 
   for (int a = me; a < taken; a += all) {
@@ -164,31 +215,27 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
     if (id < 0 || id >= p.pool_blocks) raise_status(p.status, SA_DEV_BAD_BLOCK);
     p.table[static_cast<int64_t>(b) * p.table_blocks + blocks_of(len[b]) + a - take[b]] = id;
   }
-  // Taken blocks are in the table, and every CTA has read the lengths and the
-  // list, before any of them changes.
+  // Tokens of the requests that grow by more than kFew, a warp for each chunk of one.
+  const int lane = threadIdx.x & 31;
+  for (int c = me >> 5; c < chunks; c += all >> 5) {
+    const int b = owner_of(chunk, n, c);
+    const int end = min(b + 1 < n ? tok[b + 1] : tokens, tokens);
+#pragma unroll
+    for (int k = 0; k < kChunk / 32; ++k) {
+      const int i = tok[b] + (c - chunk[b]) * kChunk + k * 32 + lane;
+      if (i < end) write_token(p, i, i - tok[b], len[b], take[b], b, top);
+    }
+  }
+  for (int i = tokens + me; i < p.max_tokens; i += all) {
+    p.slots[i] = -1;
+    if (p.positions) p.positions[i] = 0;
+  }
+  // Every CTA has read the lengths and the list before any of them changes.
   if (ctas > 1)
     cluster_barrier();
   else
     __syncthreads();
 
-  for (int i = me; i < p.max_tokens; i += all) {
-    int slot = -1, position = 0;
-    if (i < tokens) {
-      const int b = owner_of(tok, n, i);
-      const int before = len[b];
-      position = static_cast<int>(
-          min((before & 0x7fffffffll) + (i - tok[b]), 0x7fffffffll));  // far only when refused
-      if (before >= 0) {
-        const int id = p.table[static_cast<int64_t>(b) * p.table_blocks + position / kBlockTokens];
-        if (id >= 0 && id < p.pool_blocks)
-          slot = id * kBlockTokens + position % kBlockTokens;
-        else
-          raise_status(p.status, SA_DEV_BAD_BLOCK);
-      }
-    }
-    p.slots[i] = slot;
-    if (p.positions) p.positions[i] = position;
-  }
   for (int r = me; r < given; r += all) {
     const int b = owner_of(give, n, r);
     const int before = len[b] & 0x7fffffff;
@@ -213,6 +260,12 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
 }
 
 int g_plan_smem[kMaxDevices];
+bool g_plan_wide[kMaxDevices];  // clusters above the portable size allowed
+
+int plan_device() {
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < kMaxDevices ? device : 0;
+}
 
 }  // namespace
 }  // namespace sa
@@ -240,14 +293,19 @@ extern "C" SA_API sa_status sa_plan_blocks(const int32_t* add, size_t requests, 
   PlanParams p{add,       seq_lens,  block_table,   free_list, free_top,
                slots_out, positions_out, cu_tokens_out, status,    (int)requests,
                (int)table_blocks, (int)pool_blocks, (int)max_tokens};
-  // One CTA up to 4096 tokens and 1024 requests, else a cluster of 8.
+  // One CTA up to 4096 tokens and 1024 requests, else a cluster of 16.
   const bool small = max_tokens <= 4096 && requests <= 1024;
   const int threads = small && requests <= 256 && max_tokens <= 1024 ? 256 : 1024;
-  const int bytes = (int)requests * 4 * (int)sizeof(int32_t);
+  const int bytes = (int)requests * kPlanArrays * (int)sizeof(int32_t);
   const sa_status st =
       ensure_smem_limit(reinterpret_cast<const void*>(plan_kernel),
-                        kPlanMaxRequests * 4 * (int)sizeof(int32_t), g_plan_smem);
+                        kPlanMaxRequests * kPlanArrays * (int)sizeof(int32_t), g_plan_smem);
   if (st != SA_OK) return st;
+  if (!small && !g_plan_wide[plan_device()]) {
+    SA_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel),
+                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    g_plan_wide[plan_device()] = true;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(small ? 1 : kPlanCluster);
   cfg.blockDim = dim3(threads);
