@@ -210,7 +210,8 @@ SA_API size_t sa_kv4_entry_bytes(size_t head_dim);
  * followed by its inverse restores the list. A request whose growth does not
  * fit is refused: its length, blocks and table row stay, its tokens get slot
  * -1, and a status bit is set: SA_DEV_TABLE_FULL (the table's row is too
- * short), SA_DEV_SLOTS_FULL (its tokens end beyond max_tokens),
+ * short), SA_DEV_SLOTS_FULL (its last row is beyond max_tokens, be it only by
+ * the tokens of requests before it),
  * SA_DEV_POOL_EMPTY (the blocks that it and the requests before it need exceed
  * the free ones). SA_DEV_BAD_BLOCK: a length, table entry or list entry was
  * outside its range. requests <= 8192. */

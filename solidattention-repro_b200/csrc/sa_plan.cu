@@ -55,22 +55,27 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Exclusive sums of N values over the block's threads; totals get the block's.
-// narrow: over each warp's lanes alone (the warps hold the same values).
+// Sums are capped at 2^31 - 1 (a cap commutes with sums of what is not
+// negative), so that 32 bits hold them whatever the lengths.
+constexpr uint32_t kCap = 0x7fffffffu;
+__device__ __forceinline__ uint32_t add_capped(uint32_t a, uint32_t b) { return min(a + b, kCap); }
+
+// Exclusive capped sums of N values over the block's threads; totals get the
+// block's. narrow: over each warp's lanes alone (the warps hold the same values).
 template <int N>
-__device__ __forceinline__ void scan64(const long long (&value)[N], long long (&before)[N],
-                                       long long (&totals)[N], long long (*scratch)[32],
-                                       bool narrow) {
+__device__ __forceinline__ void scan(const uint32_t (&value)[N], uint32_t (&before)[N],
+                                     uint32_t (&totals)[N], uint32_t (*scratch)[32], bool narrow) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    long long sum = value[i];
+    uint32_t sum = value[i];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long n = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += n;
+      const uint32_t n = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum = add_capped(sum, n);
     }
-    before[i] = sum - value[i];
+    before[i] = __shfl_up_sync(0xffffffffu, sum, 1);
+    if (lane == 0) before[i] = 0;
     totals[i] = __shfl_sync(0xffffffffu, sum, 31);
   }
   if (narrow) return;
@@ -80,16 +85,16 @@ __device__ __forceinline__ void scan64(const long long (&value)[N], long long (&
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {  // every warp sums the warps' totals for itself
-    const long long mine = lane < warps ? scratch[i][lane] : 0;
-    long long sum = mine;
-    for (int o = 1; o < warps; o <<= 1) {
-      const long long n = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += n;
+    uint32_t sum = lane < warps ? scratch[i][lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t n = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum = add_capped(sum, n);
     }
-    totals[i] = __shfl_sync(0xffffffffu, sum, warps - 1);
-    before[i] += __shfl_sync(0xffffffffu, sum - mine, warp);
+    totals[i] = __shfl_sync(0xffffffffu, sum, 31);
+    const uint32_t mine = __shfl_sync(0xffffffffu, sum, max(warp - 1, 0));
+    if (warp > 0) before[i] = add_capped(before[i], mine);
   }
-  __syncthreads();
 }
 
 // The last index in [0, n) whose start is not above `at` (starts[0] is 0).
@@ -131,9 +136,34 @@ __device__ __forceinline__ void write_token(const PlanParams& p, int i, int k, i
   if (p.positions) p.positions[i] = position;
 }
 
+// What a step wants of a request whose new tokens start at row tok_at.
+struct Request {
+  int before, grow, held, want;  // length before, new tokens, blocks before and after
+  int rows;                      // new tokens inside the slot map
+  bool broken, full, over;
+  __device__ __forceinline__ bool refused() const { return broken || full || over; }
+  __device__ __forceinline__ bool few() const { return grow <= kFew; }
+};
+__device__ __forceinline__ Request request_of(const PlanParams& p, int b, uint32_t tok_at) {
+  const long long limit = static_cast<long long>(p.table_blocks) * kBlockTokens;
+  const int before = p.seq_lens[b], add = p.add[b];
+  Request r;
+  r.broken = before < 0 || before > limit;
+  r.before = r.broken ? 0 : before;
+  const long long after = max(0ll, static_cast<long long>(r.before) + add);
+  r.grow = max(add, 0);
+  r.full = !r.broken && after > limit;
+  const uint32_t room = max(p.max_tokens - static_cast<int>(tok_at), 0);
+  r.over = add_capped(tok_at, r.grow) > static_cast<uint32_t>(p.max_tokens);
+  r.rows = static_cast<int>(min(static_cast<uint32_t>(r.grow), room));
+  r.held = blocks_of(r.before);
+  r.want = r.refused() ? r.held : blocks_of(static_cast<int>(after));
+  return r;
+}
+
 __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
   extern __shared__ int32_t plan_smem[];
-  __shared__ long long scratch[3][32];
+  __shared__ uint32_t scratch[4][32];
   __shared__ int taken_shared;
   const int n = p.requests, rank = blockIdx.x, ctas = cluster_ctas();
   int32_t* tok = plan_smem;       // [n] first row of a request's new tokens
@@ -148,65 +178,60 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
     if (rank == 0 && threadIdx.x == 0) raise_status(p.status, SA_DEV_BAD_BLOCK);
     top = min(max(top, 0), p.pool_blocks);
   }
-  long long tok_base = 0, take_base = 0, give_base = 0, chunk_base = 0;
-  const long long limit = static_cast<long long>(p.table_blocks) * kBlockTokens;
-  const bool narrow = n <= 32;  // every warp scans all requests itself
-  for (int first = 0; first < n; first += blockDim.x) {
-    const int b = narrow ? threadIdx.x & 31 : first + threadIdx.x;
-    const bool live = b < n;
-    const int before = live ? p.seq_lens[b] : 0;
-    const int add = live ? p.add[b] : 0;
-    const bool broken = before < 0 || before > limit;
-    const long long after = broken ? 0 : max(0ll, static_cast<long long>(before) + add);
-    const long long grow = max(add, 0);
-    long long grown[1] = {grow}, grown_before[1], grown_total[1];
-    scan64(grown, grown_before, grown_total, scratch, narrow);
-    const long long tok_at = tok_base + grown_before[0];
-    tok_base += grown_total[0];
-    const bool full = !broken && after > limit;
-    const bool over = tok_at + grow > p.max_tokens;
-    bool refused = broken || full || over;
-    const int held = broken ? 0 : blocks_of(before);
-    const int want = refused ? held : blocks_of(static_cast<int>(after));
-    const int need = max(want - held, 0);
-    // blocks taken and given back (a request that gives back is not refused below)
-    const bool few = grow <= kFew;
-    // rows inside the slot map: row indices stay below max_tokens + kChunk
-    const long long rows = min(grow, max(p.max_tokens - tok_at, 0ll));
-    long long moved[3] = {need, max(held - want, 0), few ? 0 : (rows + kChunk - 1) / kChunk};
-    long long moved_before[3], moved_total[3];
-    scan64(moved, moved_before, moved_total, scratch, narrow);
-    const long long take_at = take_base + moved_before[0], give_at = give_base + moved_before[1];
-    take_base += moved_total[0];
-    give_base += moved_total[1];
-    const long long chunk_at = chunk_base + moved_before[2];
-    chunk_base += moved_total[2];
-    const bool short_of = need > 0 && take_at + need > top;
-    refused |= short_of;
-    if (need > 0 && !short_of) atomicMax(&taken_shared, static_cast<int>(take_at + need));
-    if (live) {
-      tok[b] = static_cast<int>(min(tok_at, 0x7fffffffll));
-      take[b] = static_cast<int>(min(take_at, 0x7fffffffll));
-      give[b] = static_cast<int>(give_at);
-      len[b] = (broken ? 0 : before) | (refused ? static_cast<int>(0x80000000u) : 0);
-      chunk[b] = static_cast<int>(chunk_at);
-      // requests that grow by a few tokens write them at once, those of 32 in one CTA
-      if (few && (b >> 5) % ctas == rank && (!narrow || threadIdx.x < 32))
-        for (int k = 0; k < rows; ++k)
-          write_token(p, tok[b] + k, k, len[b], take[b], b, top);
-      if (rank == 0 && (!narrow || threadIdx.x < 32)) {
-        if (broken) raise_status(p.status, SA_DEV_BAD_BLOCK);
-        if (full) raise_status(p.status, SA_DEV_TABLE_FULL);
-        if (over && !broken && !full) raise_status(p.status, SA_DEV_SLOTS_FULL);
-        if (short_of) raise_status(p.status, SA_DEV_POOL_EMPTY);
-      }
+  // A thread has `each` consecutive requests; up to 32 requests each warp has
+  // all of them and scans by itself. Lengths are read again in each pass.
+  const bool narrow = n <= 32;
+  const int each = narrow ? 1 : (n + blockDim.x - 1) / blockDim.x;
+  const int mine = narrow ? threadIdx.x & 31 : threadIdx.x * each;
+  const int mine_end = min(mine + each, n);
+  const bool speaks = !narrow || threadIdx.x < 32;  // for its requests, in this CTA
+  uint32_t grown[1] = {0}, grown_before[1], grown_total[1];
+  for (int b = mine; b < mine_end; ++b) grown[0] = add_capped(grown[0], max(p.add[b], 0));
+  scan(grown, grown_before, grown_total, scratch, narrow);
+
+  uint32_t moved[3] = {0, 0, 0}, moved_before[3], moved_total[3];  // taken, given back, chunks
+  uint32_t tok_at = grown_before[0];
+  for (int b = mine; b < mine_end; ++b) {
+    const Request r = request_of(p, b, tok_at);
+    moved[0] = add_capped(moved[0], max(r.want - r.held, 0));
+    moved[1] = add_capped(moved[1], max(r.held - r.want, 0));
+    moved[2] += r.few() ? 0 : (r.rows + kChunk - 1) / kChunk;
+    tok_at = add_capped(tok_at, r.grow);
+  }
+  scan(moved, moved_before, moved_total, scratch + 1, narrow);
+
+  tok_at = grown_before[0];
+  uint32_t take_at = moved_before[0], give_at = moved_before[1], chunk_at = moved_before[2];
+  for (int b = mine; b < mine_end; ++b) {
+    const Request r = request_of(p, b, tok_at);
+    const uint32_t need = max(r.want - r.held, 0), behind = add_capped(take_at, need);
+    const bool short_of = need > 0 && behind > static_cast<uint32_t>(top);
+    const bool refused = r.refused() || short_of;
+    if (need > 0 && !short_of) atomicMax(&taken_shared, static_cast<int>(behind));
+    tok[b] = static_cast<int>(tok_at);
+    take[b] = static_cast<int>(take_at);
+    give[b] = static_cast<int>(give_at);
+    len[b] = r.before | (refused ? static_cast<int>(0x80000000u) : 0);
+    chunk[b] = static_cast<int>(chunk_at);
+    // requests that grow by a few tokens write them at once, those of 32 in one CTA
+    if (r.few() && (b >> 5) % ctas == rank && speaks)
+      for (int k = 0; k < r.rows; ++k) write_token(p, tok[b] + k, k, len[b], take[b], b, top);
+    if (rank == 0 && speaks) {
+      if (r.broken) raise_status(p.status, SA_DEV_BAD_BLOCK);
+      if (r.full) raise_status(p.status, SA_DEV_TABLE_FULL);
+      if (r.over && !r.broken && !r.full) raise_status(p.status, SA_DEV_SLOTS_FULL);
+      if (short_of) raise_status(p.status, SA_DEV_POOL_EMPTY);
     }
+    tok_at = add_capped(tok_at, r.grow);
+    take_at = behind;
+    give_at = add_capped(give_at, max(r.held - r.want, 0));
+    chunk_at += r.few() ? 0 : (r.rows + kChunk - 1) / kChunk;
   }
   __syncthreads();
   const int taken = taken_shared;
-  const int given = static_cast<int>(min(give_base, static_cast<long long>(0x7fffffff)));
-  const int tokens = static_cast<int>(min(tok_base, static_cast<long long>(p.max_tokens)));
-  const int chunks = static_cast<int>(chunk_base);
+  const int given = static_cast<int>(moved_total[1]);
+  const int tokens = min(static_cast<int>(grown_total[0]), p.max_tokens);
+  const int chunks = static_cast<int>(moved_total[2]);
   const int me = rank * blockDim.x + threadIdx.x, all = ctas * blockDim.x;
 
   for (int a = me; a < taken; a += all) {
@@ -252,7 +277,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
       if (p.cu_tokens) p.cu_tokens[b] = tok[b];
     }
     if (threadIdx.x == 0) {
-      if (p.cu_tokens) p.cu_tokens[n] = static_cast<int>(min(tok_base, 0x7fffffffll));
+      if (p.cu_tokens) p.cu_tokens[n] = static_cast<int>(grown_total[0]);
       *p.free_top = static_cast<int>(
           min(static_cast<long long>(top) - taken + given, static_cast<long long>(p.pool_blocks)));
     }
