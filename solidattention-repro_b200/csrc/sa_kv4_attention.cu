@@ -49,7 +49,14 @@ namespace sa {
 namespace {
 
 constexpr int kMaxLists = 8192;
-constexpr int kWarps = 8;        // of an attention CTA
+// Warps of an attention CTA, one CTA an SM: 12 of 168 registers, or 8 of 255 for
+// the larger tiles. (32 requests of 8K, 8 rows a tile: 66 us with 12 warps, 73
+// with 8, 74 with two CTAs of 8 warps at 128 registers, FP32 queries 105, 107 and
+// 143; 10 and 14 warps, which the four schedulers share unevenly, 75 and 74. 16
+// rows a tile: 147 us with 8 warps, 153 with 12.)
+__host__ __device__ constexpr int attention_warps(int head_dim, int tile) {
+  return head_dim <= 128 && tile == 8 ? 12 : 8;
+}
 constexpr int kMergeWarps = 4, kMergeUnroll = 4;
 constexpr float kHeadroom = 4.0f;  // log2 by which a weight may exceed its row's running maximum
 constexpr float kWeightLog2 = 11.0f;  // weights are held as 2^11 p: at most 2^15 in FP16
@@ -73,7 +80,7 @@ struct Kv4AttnParams {
   int row_tiles;       // tiles of 8 * NT rows
   int units_per_list;  // KV heads of a list * row_tiles
   float scale_log2;    // softmax scale * log2(e)
-  int ctas;            // of the attention grid
+  int ctas, warps;     // of the attention grid, of its CTAs
   int vector_rows;     // query rows are 16-byte aligned
   int* starts;         // workspace: [lists + 1] entries of the lists before each
   float* part_ml;      // workspace: [warps][2][rows of a tile][max, sum]
@@ -234,11 +241,11 @@ __device__ __forceinline__ int list_of(const int* starts, int lists, int at) {
 struct Quota {
   int entries, cta, warp;
 };
-__device__ __forceinline__ Quota quota_of(int entries, int ctas) {
+__device__ __forceinline__ Quota quota_of(int entries, int ctas, int warps) {
   Quota q;
   q.entries = entries;
   q.cta = max((entries + ctas - 1) / ctas, 1);
-  q.warp = (q.cta + kWarps - 1) / kWarps;
+  q.warp = (q.cta + warps - 1) / warps;
   return q;
 }
 
@@ -275,8 +282,9 @@ __device__ __forceinline__ void load16(const void* base, int64_t at, bool vector
 
 // ---- attention -------------------------------------------------------------------------
 
-template <int NG>
+template <int NG, int NT>
 struct Ring {
+  static constexpr int kWarps = attention_warps(64 * NG, 8 * NT);
   static constexpr int kEntry = 36 * 64 * NG;
   static constexpr int kStages = NG == 4 ? 2 : 3;
   static constexpr int kStage = kEntry + 16;  // 16 zero bytes: the minima of lanes without a group
@@ -298,31 +306,27 @@ __device__ __forceinline__ int value_swizzle(int r) {
   return NG == 1 ? r & 2 : NG == 2 ? 2 * (r & 3) : (r & 1) | 2 * (r & 2);
 }
 
-template <int NG, int NT, int MODE>
-constexpr int min_ctas() {
-  return NG <= 2 && NT == 1 ? 2 : 1;
-}
-
 // MODE 0: 16-bit queries, BF16 output. 1: 16-bit queries, FP16 output (weights
 // in two parts). 2: FP32 queries (queries and weights in two parts).
 template <int NG, int NT, int MODE>
-__global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
+__global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
     attention_kernel(const Kv4AttnParams p) {
-  constexpr int kDim = 64 * NG, kEntry = Ring<NG>::kEntry, kStages = Ring<NG>::kStages;
+  constexpr int kWarps = Ring<NG, NT>::kWarps;
+  constexpr int kDim = 64 * NG, kEntry = Ring<NG, NT>::kEntry, kStages = Ring<NG, NT>::kStages;
   constexpr int kTile = 8 * NT;               // query rows of a unit
   constexpr int kParts = MODE == 2 ? 2 : 1;   // FP16 parts of a query
   constexpr int kWeights = MODE == 0 ? 1 : 2;  // FP16 parts of a weight
   constexpr bool kCentred = kWeights == 2;    // value codes as c - 8
   constexpr bool kCentredKeys = kParts == 2;  // key codes too
   constexpr int kPieces = kEntry / 16;        // 16-byte pieces of an entry
-  constexpr int kStage = Ring<NG>::kStage;
+  constexpr int kStage = Ring<NG, NT>::kStage;
   constexpr int kQuery = MODE == 0 ? SA_TYPE_BF16 : MODE == 1 ? SA_TYPE_F16 : SA_TYPE_F32;
   extern __shared__ __align__(128) uint8_t kv4_smem[];
   __shared__ int scan_scratch[33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  uint8_t* ring = kv4_smem + warp * Ring<NG>::kWarpBytes;
-  int* starts = reinterpret_cast<int*>(kv4_smem + Ring<NG>::kBytes);
+  uint8_t* ring = kv4_smem + warp * Ring<NG, NT>::kWarpBytes;
+  int* starts = reinterpret_cast<int*>(kv4_smem + Ring<NG, NT>::kBytes);
   const int lists = p.requests * p.lists_per_request;
   // Where a lane's 16-byte pieces of an entry go: piece 32 k + lane of the keys
   // and of the values (k even, odd), less 512 k bytes.
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
       for (int i = threadIdx.x; i <= lists; i += blockDim.x) p.starts[i] = starts[i];
   }
 
-  const Quota quota = quota_of(base * p.units_per_list, p.ctas);
+  const Quota quota = quota_of(base * p.units_per_list, p.ctas, kWarps);
   const int cta_begin = min(static_cast<int>(blockIdx.x) * quota.cta, quota.entries);
   const int cta_end = min(cta_begin + quota.cta, quota.entries);
   const int warp_begin = min(cta_begin + warp * quota.warp, cta_end);
@@ -921,11 +925,11 @@ __global__ void __launch_bounds__(kWarps * 32, min_ctas<NG, NT, MODE>())
         if (row >= p.rows) break;
         float top = -INFINITY, s = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int w = 0; w < active; ++w) {
-          const float* from = reinterpret_cast<const float*>(kv4_smem + w * Ring<NG>::kWarpBytes);
+          const float* from = reinterpret_cast<const float*>(kv4_smem + w * Ring<NG, NT>::kWarpBytes);
           top = fmaxf(top, from[kTile * kDim + r * 2]);
         }
         for (int w = 0; w < active; ++w) {
-          const float* from = reinterpret_cast<const float*>(kv4_smem + w * Ring<NG>::kWarpBytes);
+          const float* from = reinterpret_cast<const float*>(kv4_smem + w * Ring<NG, NT>::kWarpBytes);
           const float weight = exp2_approx(from[kTile * kDim + r * 2] - top);
           s = fmaf(weight, from[kTile * kDim + r * 2 + 1], s);
           const float4 v = *reinterpret_cast<const float4*>(from + r * kDim + e);
@@ -972,7 +976,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
   if (row >= p.rows) return;
   const int start = p.starts[list], n = p.starts[list + 1] - start;
   const Quota quota =
-      quota_of(p.starts[p.requests * p.lists_per_request] * p.units_per_list, p.ctas);
+      quota_of(p.starts[p.requests * p.lists_per_request] * p.units_per_list, p.ctas, p.warps);
   const int begin = start * p.units_per_list + unit * n, end = begin + n;
   // The unit's parts: those of the first CTA, one of each CTA between, those of
   // the last; a CTA whose range lies in the unit has one.
@@ -1003,7 +1007,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
       w = max(i - (ctas - 2), 0);
     }
     const bool inside = cta * quota.cta + w * quota.warp < begin;  // begins inside the warp's range
-    return ((cta * kWarps + w) * 2 + (inside ? 1 : 0)) * tile + r;
+    return ((cta * p.warps + w) * 2 + (inside ? 1 : 0)) * tile + r;
   };
   float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
   for (int i = warp; i < parts; i += kMergeWarps * kMergeUnroll) {
@@ -1070,8 +1074,9 @@ int tile_rows(size_t rows, size_t head_dim, int query_type) {
   return rows > 8 && head_dim <= 128 && query_type != SA_TYPE_F32 ? 16 : 8;
 }
 
-int max_warps(size_t head_dim, int tile) {
-  return device_sm_count() * (head_dim <= 128 && tile == 8 ? 2 : 1) * kWarps;
+// Rows of the parts that a grid of one CTA an SM may write: two units a warp.
+size_t part_rows(size_t head_dim, int tile) {
+  return (size_t)device_sm_count() * attention_warps((int)head_dim, tile) * 2 * tile;
 }
 
 size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -1080,11 +1085,11 @@ template <int NG, int NT, int MODE>
 sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
   static int configured[kMaxDevices];
   const auto kernel = attention_kernel<NG, NT, MODE>;
-  constexpr int kMost = Ring<NG>::kBytes + (kMaxLists + 1) * (int)sizeof(int);
+  constexpr int kMost = Ring<NG, NT>::kBytes + (kMaxLists + 1) * (int)sizeof(int);
   const sa_status st = ensure_smem_limit(reinterpret_cast<const void*>(kernel), kMost, configured);
   if (st != SA_OK) return st;
-  const size_t smem = Ring<NG>::kBytes + (size_t)(lists + 1) * sizeof(int);
-  SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(kWarps * 32), smem, stream, false, p));
+  const size_t smem = Ring<NG, NT>::kBytes + (size_t)(lists + 1) * sizeof(int);
+  SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(Ring<NG, NT>::kWarps * 32), smem, stream, false, p));
   const int rows = std::min(p.rows, 8 * NT);
   return cuda_status(launch_kernel(merge_kernel<NG>, dim3(lists * p.units_per_list * rows),
                                    dim3(kMergeWarps * 32), 0, stream, false, p, 8 * NT),
@@ -1118,11 +1123,8 @@ extern "C" SA_API size_t sa_attention_kv4_workspace_size(size_t requests, size_t
   if (requests == 0 || new_tokens == 0 || kv_heads == 0 || query_heads == 0 ||
       query_heads % kv_heads != 0 || sa_kv4_entry_bytes(head_dim) == 0)
     return 0;
-  // starts of up to kMaxLists lists, two parts a warp: the same bytes for 8
-  // rows on twice the warps as for 16
-  const size_t rows = (size_t)max_warps(head_dim, 8) * 2 * 8;
-  return round256((kMaxLists + 1) * sizeof(int)) + rows * 2 * sizeof(float) +
-         rows * head_dim * sizeof(float);
+  const size_t rows = std::max(part_rows(head_dim, 8), part_rows(head_dim, 16));
+  return round256((kMaxLists + 1) * sizeof(int)) + rows * (2 + head_dim) * sizeof(float);
 }
 
 extern "C" SA_API sa_status sa_attention_kv4(
@@ -1203,12 +1205,12 @@ extern "C" SA_API sa_status sa_attention_kv4(
   const size_t element = query_type == SA_TYPE_F32 ? 4 : 2;
   p.vector_rows = ((reinterpret_cast<uintptr_t>(query) | (size_t)stride_request * element |
                     (size_t)stride_token * element | (size_t)stride_head * element) & 15u) == 0;
-  p.ctas = max_warps(head_dim, tile) / kWarps;
-  const size_t part_rows = (size_t)p.ctas * kWarps * 2 * tile;
+  p.ctas = device_sm_count();
+  p.warps = attention_warps((int)head_dim, tile);
   char* ws = static_cast<char*>(workspace);
   p.starts = reinterpret_cast<int*>(ws);
   p.part_ml = reinterpret_cast<float*>(ws + round256((kMaxLists + 1) * sizeof(int)));
-  p.part_o = p.part_ml + part_rows * 2;
+  p.part_o = p.part_ml + part_rows(head_dim, tile) * 2;
   const int all = (int)(requests * lists);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return head_dim == 64    ? launch_dim<1>(p, all, tile, s)
