@@ -958,73 +958,65 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
   }
 }
 
-// Joins the parts of split units and writes the rows of empty ones: one CTA a
-// query row, its warps sharing the parts.
-template <int NG>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnParams p, int tile) {
-  constexpr int kDim = 64 * NG, kPerLane = kDim / 32;
-  __shared__ float shared_o[kMergeWarps][kDim];
-  __shared__ float shared_ml[kMergeWarps][2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows = min(tile, p.rows);
-  const int r = blockIdx.x % rows, u = blockIdx.x / rows;
-  const int list = u / p.units_per_list, unit = u % p.units_per_list;
-  const int b = list / p.lists_per_request;
-  const int kv_head =
-      list % p.lists_per_request * (p.kv_heads / p.lists_per_request) + unit / p.row_tiles;
-  const int row = unit % p.row_tiles * tile + r;
-  if (row >= p.rows) return;
-  const int start = p.starts[list], n = p.starts[list + 1] - start;
-  const Quota quota =
-      quota_of(p.starts[p.requests * p.lists_per_request] * p.units_per_list, p.ctas, p.warps);
-  const int begin = start * p.units_per_list + unit * n, end = begin + n;
-  // The unit's parts: those of the first CTA, one of each CTA between, those of
-  // the last; a CTA whose range lies in the unit has one.
-  int first = 0, parts = 0, first_parts = 0, last_warp = 0, first_warp = 0, ctas = 0;
-  if (n > 0) {
-    first = begin / quota.cta;
-    const int last = (end - 1) / quota.cta;
-    ctas = last - first + 1;
-    const auto covers = [&](int cta) {
-      return begin <= cta * quota.cta && end >= min((cta + 1) * quota.cta, quota.entries);
-    };
-    if (!covers(first)) first_warp = (begin - first * quota.cta) / quota.warp;
-    first_parts = covers(first) ? 1
-                                : (min(end - first * quota.cta, quota.cta) - 1) / quota.warp -
-                                      first_warp + 1;
-    parts = first_parts;
-    if (ctas > 1) {
-      last_warp = covers(last) ? 0 : (end - 1 - last * quota.cta) / quota.warp;
-      parts += ctas - 2 + last_warp + 1;
-    }
-    if (parts == 1) return;  // written by the attention
-  }
-  const auto slot = [&](int i) {  // row r of part i
-    int cta = first, w = first_warp + i;
-    if (i >= first_parts) {
-      i -= first_parts;
-      cta = first + 1 + min(i, ctas - 2);
-      w = max(i - (ctas - 2), 0);
-    }
-    const bool inside = cta * quota.cta + w * quota.warp < begin;  // begins inside the warp's range
-    return ((cta * p.warps + w) * 2 + (inside ? 1 : 0)) * tile + r;
+// Where the parts of a unit [begin, end) of the flat list are: those of the
+// first CTA's warps, one of each CTA between, those of the last CTA's; a CTA
+// whose whole range lies in the unit has one, its warp 0's.
+struct Parts {
+  int begin, first, first_warp, first_parts, ctas, count;
+};
+__device__ __forceinline__ Parts parts_of(const Quota& q, int begin, int end) {
+  Parts u{};
+  u.begin = begin;
+  if (begin == end) return u;
+  u.first = begin / q.cta;
+  const int last = (end - 1) / q.cta;
+  u.ctas = last - u.first + 1;
+  const auto covers = [&](int cta) {
+    return begin <= cta * q.cta && end >= min((cta + 1) * q.cta, q.entries);
   };
-  float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
-  for (int i = warp; i < parts; i += kMergeWarps * kMergeUnroll) {
+  u.first_warp = (begin - u.first * q.cta) / q.warp;
+  u.first_parts = covers(u.first)
+                      ? 1
+                      : (min(end - u.first * q.cta, q.cta) - 1) / q.warp - u.first_warp + 1;
+  u.count = u.first_parts;
+  if (u.ctas > 1) u.count += u.ctas - 1 + (covers(last) ? 0 : (end - 1 - last * q.cta) / q.warp);
+  return u;
+}
+// Slot of a unit's i-th part.
+__device__ __forceinline__ int part_slot(const Parts& u, const Quota& q, int warps, int i) {
+  int cta = u.first, w = u.first_warp + i;
+  if (i >= u.first_parts) {
+    i -= u.first_parts;
+    cta = u.first + 1 + min(i, u.ctas - 2);
+    w = max(i - (u.ctas - 2), 0);
+  }
+  const bool inside = cta * q.cta + w * q.warp < u.begin;  // begins inside the warp's range
+  return (cta * warps + w) * 2 + (inside ? 1 : 0);
+}
+
+// Joins parts first, first + stride, ... of row r of a unit in one warp: lane l
+// gets elements l, l + 32, ...
+template <int NG>
+__device__ __forceinline__ void join_parts(const Kv4AttnParams& p, const Quota& q, const Parts& u,
+                                           int tile, int r, int first, int stride, float& top,
+                                           float& sum, float (&o)[2 * NG]) {
+  constexpr int kDim = 64 * NG, kPerLane = 2 * NG;
+  const int lane = threadIdx.x & 31;
+  for (int i = first; i < u.count; i += stride * kMergeUnroll) {
     float ml[kMergeUnroll][2], v[kMergeUnroll][kPerLane];
 #pragma unroll
     for (int k = 0; k < kMergeUnroll; ++k) {
-      const int at = slot(min(i + k * kMergeWarps, parts - 1));
-      const float2 pair = *reinterpret_cast<const float2*>(p.part_ml + static_cast<int64_t>(at) * 2);
+      const int64_t at =
+          static_cast<int64_t>(part_slot(u, q, p.warps, min(i + k * stride, u.count - 1))) * tile + r;
+      const float2 pair = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
       ml[k][0] = pair.x;
       ml[k][1] = pair.y;
 #pragma unroll
-      for (int j = 0; j < kPerLane; ++j)
-        v[k][j] = p.part_o[static_cast<int64_t>(at) * kDim + j * 32 + lane];
+      for (int j = 0; j < kPerLane; ++j) v[k][j] = p.part_o[at * kDim + j * 32 + lane];
     }
 #pragma unroll
     for (int k = 0; k < kMergeUnroll; ++k) {
-      if (i + k * kMergeWarps >= parts) break;
+      if (i + k * stride >= u.count) break;
       const float now = fmaxf(top, ml[k][0]);
       const float keep = exp2_approx(top - now), weight = exp2_approx(ml[k][0] - now);
       top = now;
@@ -1033,36 +1025,81 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
       for (int j = 0; j < kPerLane; ++j) o[j] = fmaf(o[j], keep, weight * v[k][j]);
     }
   }
-  if (lane == 0) {
-    shared_ml[warp][0] = top;
-    shared_ml[warp][1] = sum;
-  }
+}
+
+__device__ __forceinline__ void store1(void* base, int64_t i, int type, float x) {
+  if (type == SA_TYPE_F32)
+    static_cast<float*>(base)[i] = x;
+  else if (type == SA_TYPE_F16)
+    static_cast<__half*>(base)[i] = __float2half_rn(x);
+  else
+    static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
+}
+
+// Joins the parts of split units and writes the rows of empty ones. MANY = 0:
+// one CTA a query row, its warps sharing the row's parts, of which few units can
+// have hundreds. MANY = 1: one CTA a unit, a warp a row, for batches of many
+// short units, most of them written already (512 requests of 100 tokens: 66 us
+// with a CTA a row).
+template <int NG, int MANY>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnParams p, int tile) {
+  constexpr int kDim = 64 * NG, kPerLane = kDim / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = min(tile, p.rows);
+  const int u = MANY ? blockIdx.x : blockIdx.x / rows;
+  const int list = u / p.units_per_list, unit = u % p.units_per_list;
+  const int start = p.starts[list], n = p.starts[list + 1] - start;
+  const Quota quota =
+      quota_of(p.starts[p.requests * p.lists_per_request] * p.units_per_list, p.ctas, p.warps);
+  const int begin = start * p.units_per_list + unit * n;
+  const Parts parts = parts_of(quota, begin, begin + n);
+  if (parts.count == 1) return;  // written by the attention
+  const int b = list / p.lists_per_request;
+  const int kv_head =
+      list % p.lists_per_request * (p.kv_heads / p.lists_per_request) + unit / p.row_tiles;
+  const int row0 = unit % p.row_tiles * tile;
+  if constexpr (MANY) {
+    for (int r = warp; r < rows && row0 + r < p.rows; r += kMergeWarps) {
+      float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
+      join_parts<NG>(p, quota, parts, tile, r, 0, 1, top, sum, o);
+      const int64_t out_row = output_row(p, b, kv_head, row0 + r);
+      const float scale = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
-  for (int j = 0; j < kPerLane; ++j) shared_o[warp][j * 32 + lane] = o[j];
-  __syncthreads();
-  top = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, shared_ml[w][0]);
-  const int64_t out_row = output_row(p, b, kv_head, row);
-  for (int e = threadIdx.x; e < kDim; e += kMergeWarps * 32) {
-    float y = 0.0f;
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) {
-      if (w >= parts) break;
-      const float weight = exp2_approx(shared_ml[w][0] - top);
-      sum = fmaf(weight, shared_ml[w][1], sum);
-      y = fmaf(weight, shared_o[w][e], y);
+      for (int j = 0; j < kPerLane; ++j)
+        store1(p.out, out_row * kDim + j * 32 + lane, p.out_type, o[j] * scale);
+      if (p.lse && lane == 0) p.lse[out_row] = log_of_sum(top, sum);
     }
-    y = sum != 0.0f ? y / sum : 0.0f;
-    const int64_t at = out_row * kDim + e;
-    if (p.out_type == SA_TYPE_F32)
-      static_cast<float*>(p.out)[at] = y;
-    else if (p.out_type == SA_TYPE_F16)
-      static_cast<__half*>(p.out)[at] = __float2half_rn(y);
-    else
-      static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
-    if (p.lse && e == 0) p.lse[out_row] = log_of_sum(top, sum);
+  } else {
+    __shared__ float shared_o[kMergeWarps][kDim];
+    __shared__ float shared_ml[kMergeWarps][2];
+    const int r = blockIdx.x % rows;
+    if (row0 + r >= p.rows) return;
+    float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
+    join_parts<NG>(p, quota, parts, tile, r, warp, kMergeWarps, top, sum, o);
+    if (lane == 0) {
+      shared_ml[warp][0] = top;
+      shared_ml[warp][1] = sum;
+    }
+#pragma unroll
+    for (int j = 0; j < kPerLane; ++j) shared_o[warp][j * 32 + lane] = o[j];
+    __syncthreads();
+    top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, shared_ml[w][0]);
+    const int64_t out_row = output_row(p, b, kv_head, row0 + r);
+    for (int e = threadIdx.x; e < kDim; e += kMergeWarps * 32) {
+      float y = 0.0f;
+      sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kMergeWarps; ++w) {
+        if (w >= parts.count) break;
+        const float weight = exp2_approx(shared_ml[w][0] - top);
+        sum = fmaf(weight, shared_ml[w][1], sum);
+        y = fmaf(weight, shared_o[w][e], y);
+      }
+      store1(p.out, out_row * kDim + e, p.out_type, sum != 0.0f ? y / sum : 0.0f);
+      if (p.lse && e == 0) p.lse[out_row] = log_of_sum(top, sum);
+    }
   }
 }
 
@@ -1090,10 +1127,14 @@ sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
   if (st != SA_OK) return st;
   const size_t smem = Ring<NG, NT>::kBytes + (size_t)(lists + 1) * sizeof(int);
   SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(Ring<NG, NT>::kWarps * 32), smem, stream, false, p));
-  const int rows = std::min(p.rows, 8 * NT);
-  return cuda_status(launch_kernel(merge_kernel<NG>, dim3(lists * p.units_per_list * rows),
-                                   dim3(kMergeWarps * 32), 0, stream, false, p, 8 * NT),
-                     "attention_kv4 merge launch");
+  const int units = lists * p.units_per_list;
+  const cudaError_t err =
+      units > 4 * p.ctas
+          ? launch_kernel(merge_kernel<NG, 1>, dim3(units), dim3(kMergeWarps * 32), 0, stream, false,
+                          p, 8 * NT)
+          : launch_kernel(merge_kernel<NG, 0>, dim3(units * std::min(p.rows, 8 * NT)),
+                          dim3(kMergeWarps * 32), 0, stream, false, p, 8 * NT);
+  return cuda_status(err, "attention_kv4 merge launch");
 }
 
 template <int NG>
