@@ -128,10 +128,18 @@ struct Row16 {
 #pragma unroll
     for (int i = 0; i < 8; ++i) word[i] = 0u;
   }
-  __device__ __forceinline__ float value(int i) const {
-    const uint32_t w = word[i >> 1];
-    if constexpr (TYPE == SA_TYPE_BF16) return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
-    return h2f(static_cast<uint16_t>(i & 1 ? w >> 16 : w));
+  __device__ __forceinline__ void values(float (&x)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (TYPE == SA_TYPE_BF16) {
+        x[2 * i] = __uint_as_float(word[i] << 16);
+        x[2 * i + 1] = __uint_as_float(word[i] & 0xffff0000u);
+      } else {
+        const float2 f = h2x2f(word[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
   }
   __device__ __forceinline__ void limits(float& low, float& high) const {
     Pair a = pair(0), b = a;
@@ -169,7 +177,10 @@ struct Row16<SA_TYPE_F32> {
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = 0.0f;
   }
-  __device__ __forceinline__ float value(int i) const { return x[i]; }
+  __device__ __forceinline__ void values(float (&y)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) y[i] = x[i];
+  }
   __device__ __forceinline__ void limits(float& low, float& high) const {
     low = high = x[0];
 #pragma unroll
@@ -212,8 +223,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams p) {
     }
     const bool finite = low >= -FLT_MAX && high <= FLT_MAX;
     float x[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = row[i].value(e);
+    row[i].values(x);
     if (TYPE != SA_TYPE_F16 && (low < -65504.0f || high > 65504.0f)) {
       low = fminf(fmaxf(low, -65504.0f), 65504.0f);
       high = fminf(fmaxf(high, -65504.0f), 65504.0f);

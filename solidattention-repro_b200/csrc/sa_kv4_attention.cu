@@ -49,13 +49,13 @@ namespace sa {
 namespace {
 
 constexpr int kMaxLists = 8192;
-// Warps of an attention CTA, one CTA an SM: 12 of 168 registers, or 8 of 255 for
-// the larger tiles. (32 requests of 8K, 8 rows a tile: 66 us with 12 warps, 73
+// Warps of an attention CTA, one CTA an SM: 16 of 128 registers, 12 of 168, or 8
+// of 255 for the larger tiles. (32 requests of 8K, 8 rows a tile: 66 us with 12 warps, 73
 // with 8, 74 with two CTAs of 8 warps at 128 registers, FP32 queries 105, 107 and
 // 143; 10 and 14 warps, which the four schedulers share unevenly, 75 and 74. 16
 // rows a tile: 147 us with 8 warps, 153 with 12.)
 __host__ __device__ constexpr int attention_warps(int head_dim, int tile) {
-  return head_dim <= 128 && tile == 8 ? 12 : 8;
+  return tile > 8 || head_dim > 128 ? 8 : head_dim == 64 ? 16 : 12;
 }
 constexpr int kMergeWarps = 4, kMergeUnroll = 4;
 constexpr float kHeadroom = 4.0f;  // log2 by which a weight may exceed its row's running maximum
