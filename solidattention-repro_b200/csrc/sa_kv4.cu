@@ -24,7 +24,7 @@
 namespace sa {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kTokens = 2;  // consecutive tokens of a thread
 
 struct PackParams {

@@ -27,34 +27,35 @@ from ._lib import SA_TYPE_BF16, SA_TYPE_F16, SA_TYPE_F32, check, load
 _TYPES = {torch.float32: SA_TYPE_F32, torch.float16: SA_TYPE_F16, torch.bfloat16: SA_TYPE_BF16}
 
 
-def _tensor(t, dtype, dim, name, device=None) -> int:
-    """The address of a contiguous CUDA tensor of the given type and rank."""
+def _tensor(t, dtype, dim, name, index=None) -> int:
+    """The address of a contiguous CUDA tensor of the given type and rank (on
+    device `index`)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != dim or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous with {dim} dimension(s)")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if index is not None and t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
     return t.data_ptr()
 
 
-def _rows(t, dim, name, device) -> int:
+def _rows(t, dim, name, index) -> int:
     """The address of a CUDA tensor whose last axis is contiguous."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype not in _TYPES:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    if t.dim() != dim or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name} must have {dim} dimensions, the last one contiguous")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
     return t.data_ptr()
 
 
-def _status(status, device):
-    return None if status is None else _tensor(status, torch.int32, 1, "status", device)
+def _status(status, index):
+    return None if status is None else _tensor(status, torch.int32, 1, "status", index)
 
 
 def _public_stream(index: int) -> int:
@@ -65,13 +66,12 @@ def _public_stream(index: int) -> int:
 _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
-def _call(device, what, fn, *args) -> None:
-    """fn(*args, stream) with the current stream of `device`, made current for the call."""
-    index = device.index
+def _call(index, what, fn, *args) -> None:
+    """fn(*args, stream) with the current stream of device `index`, made current for the call."""
     if index == torch.cuda.current_device():
         status = fn(*args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = fn(*args, _stream_of(index))
     if status:
         check(status, what)
@@ -110,7 +110,7 @@ def plan_blocks(add: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Te
     (sa_plan_blocks).
     """
     ptr = _tensor(add, torch.int32, 1, "add")
-    dev = add.device
+    dev = add.get_device()
     n = add.shape[0]
     lens = _tensor(seq_lens, torch.int32, 1, "seq_lens", dev)
     table = _tensor(block_table, torch.int32, 2, "block_table", dev)
@@ -134,7 +134,7 @@ def pack_kv4(pool: torch.Tensor, key: torch.Tensor, value: torch.Tensor, slots: 
     ``slots`` [tokens] int32 of ``pool``; rows with a negative slot are skipped
     (sa_pack_kv4)."""
     ptr, blocks, heads, d = _pool_dims(pool)
-    dev = pool.device
+    dev = pool.get_device()
     k, v = _rows(key, 3, "key", dev), _rows(value, 3, "value", dev)
     at = _tensor(slots, torch.int32, 1, "slots", dev)
     tokens = slots.shape[0]
@@ -150,13 +150,13 @@ def unpack_kv4(pool: torch.Tensor, slots: torch.Tensor, dtype: torch.dtype = tor
     """The rows held in ``slots`` [tokens] int32: (key, value) [tokens, kv_heads,
     head_dim] of ``dtype``, zeros where the slot is negative (sa_unpack_kv4)."""
     ptr, blocks, heads, d = _pool_dims(pool)
-    dev = pool.device
+    dev = pool.get_device()
     at = _tensor(slots, torch.int32, 1, "slots", dev)
     if dtype not in _TYPES:
         raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     tokens = slots.shape[0]
-    key = torch.empty(tokens, heads, d, dtype=dtype, device=dev)
-    value = key.new_empty(key.shape)
+    key = pool.new_empty((tokens, heads, d), dtype=dtype)
+    value = key.new_empty((tokens, heads, d))
     _call(dev, "unpack_kv4", load().sa_unpack_kv4, ptr, blocks, at, tokens, heads, d, key.data_ptr(),
           value.data_ptr(), _TYPES[dtype], _status(status, dev))
     return key, value
@@ -188,7 +188,7 @@ def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Te
     log-sum-exp of the logits, FP32, without head_dim (sa_attention_kv4).
     """
     ptr, blocks, heads, d = _pool_dims(pool)
-    dev = pool.device
+    dev = pool.get_device()
     lead = 4 if isinstance(query, torch.Tensor) and query.dim() == 4 else 3
     q = _rows(query, lead, "query", dev)
     n, qh = query.shape[0], query.shape[-2]
@@ -212,11 +212,12 @@ def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Te
     out_dtype = query.dtype if out_dtype is None else out_dtype
     if out_dtype not in _TYPES:
         raise TypeError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    out = query.new_empty(query.shape, dtype=out_dtype)
-    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=dev) if return_lse else None
+    shape = query.shape
+    out = query.new_empty(shape, dtype=out_dtype)
+    lse = query.new_empty(shape[:-1], dtype=torch.float32) if return_lse else None
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    ws_bytes = _workspace_bytes(n, new, qh, heads, d, dev.index)
+    ws_bytes = _workspace_bytes(n, new, qh, heads, d, dev)
     ws = pool.new_empty(ws_bytes or 16)
     _call(dev, "attention_kv4", lib.sa_attention_kv4, q, _TYPES[query.dtype], query.stride(0),
           query.stride(1) if lead == 4 else 0, query.stride(-2), ptr, blocks, table,
