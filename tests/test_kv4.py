@@ -792,3 +792,99 @@ def test_selection_from_the_cache(pkg, cuda):
     packed = torch.stack([kk[:, :1], vv[:, :1]], 1).contiguous()
     near = pkg.attention(packed, q[0, :group].contiguous(), len(where), group, 1, d)
     torch.testing.assert_close(out[0, :group], near, rtol=0, atol=2e-3)
+
+
+@pytest.mark.gpu
+def test_calls_at_once_on_two_streams_and_from_two_graphs(pkg, cuda):
+    """Attention over different caches in flight together: each call has a workspace of its own."""
+    rng = np.random.default_rng(41)
+    cases = []
+    for lens in ([5000, 40, 0, 700], [33, 6000, 1200]):
+        pool, table = _cache(rng, len(lens), lens, 2, 128, cuda)
+        q = _query(rng, (len(lens), 8, 128), torch.float32, cuda)
+        cases.append([q, torch.as_tensor(pool, device=cuda), _i32(table, cuda), _i32(lens, cuda)])
+    want = [pkg.attention_kv4(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(cuda) for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(pkg.attention_kv4(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+    graphs, outs = [], []
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(pkg.attention_kv4(*c))
+        graphs.append(graph)
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
+@pytest.mark.gpu
+def test_a_layer_of_a_larger_tensor_and_a_broadcast_query(pkg, cuda):
+    """Pools as slices of one tensor of all layers; a query with stride 0 over the requests."""
+    rng = np.random.default_rng(42)
+    lens = [90, 33]
+    pool, table = _cache(rng, 2, lens, 2, 64, cuda)
+    layers = torch.zeros(3, *pool.shape, dtype=torch.uint8, device=cuda)
+    layers[1] = torch.as_tensor(pool, device=cuda)
+    q = _query(rng, (1, 4, 64), torch.float16, cuda).expand(2, 4, 64)
+    out = pkg.attention_kv4(q, layers[1], _i32(table, cuda), _i32(lens, cuda))
+    assert torch.equal(out, _check(pkg, q, pool, table, lens, cuda))
+    assert (layers[0] == 0).all() and (layers[2] == 0).all()
+
+
+@pytest.mark.gpu
+def test_results_do_not_depend_on_the_run(pkg, cuda):
+    """No atomics in any sum: the same call gives the same bytes."""
+    rng = np.random.default_rng(43)
+    lens = [int(x) for x in rng.integers(0, 4000, 24)]
+    pool, table = _cache(rng, 24, lens, 2, 128, cuda)
+    dev = [torch.as_tensor(pool, device=cuda), _i32(table, cuda), _i32(lens, cuda)]
+    for dtype in TYPES:
+        q = _query(rng, (24, 3, 8, 128), dtype, cuda)
+        first = pkg.attention_kv4(q, *dev, return_lse=True)
+        for _ in range(5):
+            again = pkg.attention_kv4(q, *dev, return_lse=True)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.gpu
+def test_one_long_request_among_many_short_ones(pkg, cuda):
+    """A unit in hundreds of parts in a batch of many units; the others in one part or none."""
+    gen = torch.Generator(device=cuda).manual_seed(44)
+    n, kh, d, longest = 400, 2, 128, 30000
+    lens = np.full(n, 3)
+    lens[::7] = 0
+    lens[200] = longest
+    held = -(-lens // 32)
+    total = int(held.sum())
+    pool = pkg.kv4_pool(total, kh, d, device=cuda)
+    x = torch.randn(2, total * 32, kh, d, generator=gen, device=cuda)
+    pkg.pack_kv4(pool, x[0], x[1], torch.arange(total * 32, dtype=torch.int32, device=cuda))
+    table = np.full((n, int(held.max())), -1)
+    ends = np.cumsum(held)
+    for b in range(n):
+        table[b, :held[b]] = np.arange(ends[b] - held[b], ends[b])
+    q = torch.randn(n, 4, d, generator=gen, device=cuda)
+    out, lse = pkg.attention_kv4(q, pool, _i32(table, cuda), _i32(lens, cuda), return_lse=True)
+    assert (out[::7] == 0).all() and torch.isneginf(lse[::7]).all()
+    for b in (1, 199, 200, 201, 399):
+        slots = torch.arange(int(lens[b]), dtype=torch.int32, device=cuda) + 32 * int(ends[b] - held[b])
+        k, v = (t.double() for t in pkg.unpack_kv4(pool, slots, torch.float32))
+        s = torch.einsum("hgd,thd->hgt", q[b].double().view(kh, 2, d), k) / math.sqrt(d)
+        want = torch.einsum("hgt,thd->hgd", torch.softmax(s, -1), v).reshape(4, d)
+        # as in test_attention_batches: |v| up to 6, a logit summed from up to 60
+        assert float((out[b].double() - want).abs().max()) <= 6 * (2.0 ** -20 * 60 + 2.0 ** -19)
