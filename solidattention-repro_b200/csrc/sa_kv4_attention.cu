@@ -63,7 +63,6 @@ constexpr int kMaxLists = 8192;
 __host__ __device__ constexpr int attention_warps(int head_dim, int tile) {
   return tile > 8 || head_dim > 128 ? 8 : head_dim == 64 ? 16 : 12;
 }
-constexpr int kMergeWarps = 4, kMergeUnroll = 4;
 constexpr float kHeadroom = 4.0f;  // log2 by which a weight may exceed its row's running maximum
 constexpr float kWeightLog2 = 11.0f;  // weights are held as 2^11 p: at most 2^15 in FP16
 
@@ -1001,17 +1000,17 @@ __device__ __forceinline__ int part_slot(const Parts& u, const Quota& q, int war
 }
 
 // Joins parts first, first + stride, ... of row r of a unit in one warp: lane l
-// gets elements l, l + 32, ...
-template <int NG>
+// gets elements l, l + 32, ...; UNROLL parts' loads are in flight together.
+template <int NG, int UNROLL>
 __device__ __forceinline__ void join_parts(const Kv4AttnParams& p, const Quota& q, const Parts& u,
                                            int tile, int r, int first, int stride, float& top,
                                            float& sum, float (&o)[2 * NG]) {
   constexpr int kDim = 64 * NG, kPerLane = 2 * NG;
   const int lane = threadIdx.x & 31;
-  for (int i = first; i < u.count; i += stride * kMergeUnroll) {
-    float ml[kMergeUnroll][2], v[kMergeUnroll][kPerLane];
+  for (int i = first; i < u.count; i += stride * UNROLL) {
+    float ml[UNROLL][2], v[UNROLL][kPerLane];
 #pragma unroll
-    for (int k = 0; k < kMergeUnroll; ++k) {
+    for (int k = 0; k < UNROLL; ++k) {
       const int64_t at =
           static_cast<int64_t>(part_slot(u, q, p.warps, min(i + k * stride, u.count - 1))) * tile + r;
       const float2 pair = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
@@ -1021,7 +1020,7 @@ __device__ __forceinline__ void join_parts(const Kv4AttnParams& p, const Quota& 
       for (int j = 0; j < kPerLane; ++j) v[k][j] = p.part_o[at * kDim + j * 32 + lane];
     }
 #pragma unroll
-    for (int k = 0; k < kMergeUnroll; ++k) {
+    for (int k = 0; k < UNROLL; ++k) {
       if (i + k * stride >= u.count) break;
       const float now = fmaxf(top, ml[k][0]);
       const float keep = exp2_approx(top - now), weight = exp2_approx(ml[k][0] - now);
@@ -1042,17 +1041,17 @@ __device__ __forceinline__ void store1(void* base, int64_t i, int type, float x)
     static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
 }
 
-// Joins the parts of split units and writes the rows of empty ones. MANY = 0:
-// one CTA a query row, its warps sharing the row's parts, of which few units can
-// have hundreds. MANY = 1: one CTA a unit, a warp a row, for batches of many
-// short units, most of them written already (512 requests of 100 tokens: 66 us
-// with a CTA a row).
-template <int NG, int MANY>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnParams p, int tile) {
+// Joins the parts of split units and writes the rows of empty ones. SHARED: one
+// CTA a query row, its warps sharing the row's parts, of which few units can have
+// hundreds. Otherwise one CTA a unit and a warp a row: most of the cost is then
+// finding the parts, and many units have none left to join (512 requests of 100
+// tokens: 66 us with a CTA a row, 46 us so).
+template <int NG, int WARPS, bool SHARED>
+__global__ void __launch_bounds__(WARPS * 32) merge_kernel(const Kv4AttnParams p, int tile) {
   constexpr int kDim = 64 * NG, kPerLane = kDim / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = min(tile, p.rows);
-  const int u = MANY ? blockIdx.x : blockIdx.x / rows;
+  const int u = SHARED ? blockIdx.x / rows : blockIdx.x;
   const int list = u / p.units_per_list, unit = u % p.units_per_list;
   const int start = p.starts[list], n = p.starts[list + 1] - start;
   const Quota quota =
@@ -1064,10 +1063,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
   const int kv_head =
       list % p.lists_per_request * (p.kv_heads / p.lists_per_request) + unit / p.row_tiles;
   const int row0 = unit % p.row_tiles * tile;
-  if constexpr (MANY) {
-    for (int r = warp; r < rows && row0 + r < p.rows; r += kMergeWarps) {
+  if constexpr (!SHARED) {
+    for (int r = warp; r < rows && row0 + r < p.rows; r += WARPS) {
       float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
-      join_parts<NG>(p, quota, parts, tile, r, 0, 1, top, sum, o);
+      join_parts<NG, 8>(p, quota, parts, tile, r, 0, 1, top, sum, o);
       const int64_t out_row = output_row(p, b, kv_head, row0 + r);
       const float scale = sum != 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
@@ -1076,12 +1075,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
       if (p.lse && lane == 0) p.lse[out_row] = log_of_sum(top, sum);
     }
   } else {
-    __shared__ float shared_o[kMergeWarps][kDim];
-    __shared__ float shared_ml[kMergeWarps][2];
+    __shared__ float shared_o[WARPS][kDim];
+    __shared__ float shared_ml[WARPS][2];
     const int r = blockIdx.x % rows;
     if (row0 + r >= p.rows) return;
     float top = -INFINITY, sum = 0.0f, o[kPerLane] = {};
-    join_parts<NG>(p, quota, parts, tile, r, warp, kMergeWarps, top, sum, o);
+    join_parts<NG, 4>(p, quota, parts, tile, r, warp, WARPS, top, sum, o);
     if (lane == 0) {
       shared_ml[warp][0] = top;
       shared_ml[warp][1] = sum;
@@ -1091,13 +1090,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const Kv4AttnPa
     __syncthreads();
     top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, shared_ml[w][0]);
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, shared_ml[w][0]);
     const int64_t out_row = output_row(p, b, kv_head, row0 + r);
-    for (int e = threadIdx.x; e < kDim; e += kMergeWarps * 32) {
+    for (int e = threadIdx.x; e < kDim; e += WARPS * 32) {
       float y = 0.0f;
       sum = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kMergeWarps; ++w) {
+      for (int w = 0; w < WARPS; ++w) {
         if (w >= parts.count) break;
         const float weight = exp2_approx(shared_ml[w][0] - top);
         sum = fmaf(weight, shared_ml[w][1], sum);
@@ -1133,13 +1132,17 @@ sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
   if (st != SA_OK) return st;
   const size_t smem = Ring<NG, NT>::kBytes + (size_t)(lists + 1) * sizeof(int);
   SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(Ring<NG, NT>::kWarps * 32), smem, stream, false, p));
-  const int units = lists * p.units_per_list;
-  const cudaError_t err =
-      units > 4 * p.ctas
-          ? launch_kernel(merge_kernel<NG, 1>, dim3(units), dim3(kMergeWarps * 32), 0, stream, false,
-                          p, 8 * NT)
-          : launch_kernel(merge_kernel<NG, 0>, dim3(units * std::min(p.rows, 8 * NT)),
-                          dim3(kMergeWarps * 32), 0, stream, false, p, 8 * NT);
+  // A warp a row where units have some four parts (all warps' ranges over the
+  // units), else a CTA a row: 16, 32 and 64 requests of 8K (14, 7 and 3.5 parts)
+  // took 44, 67 and 116 us with a CTA a row, 49, 68 and 114 us with a warp.
+  const int units = lists * p.units_per_list, rows = std::min(p.rows, 8 * NT);
+  const auto merge = [&](auto kernel_, int grid, int warps) {
+    return launch_kernel(kernel_, dim3(grid), dim3(warps * 32), 0, stream, false, p, 8 * NT);
+  };
+  const cudaError_t err = units < p.ctas * p.warps / 4 ? merge(merge_kernel<NG, 4, true>, units * rows, 4)
+                          : rows <= 4                   ? merge(merge_kernel<NG, 4, false>, units, 4)
+                          : rows <= 8                   ? merge(merge_kernel<NG, 8, false>, units, 8)
+                                                        : merge(merge_kernel<NG, 16, false>, units, 16);
   return cuda_status(err, "attention_kv4 merge launch");
 }
 
