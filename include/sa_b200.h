@@ -258,7 +258,7 @@ SA_API sa_status sa_unpack_kv4(const void* pool, size_t pool_blocks,
  *         that sees none gives zeros (and -inf in lse_out).
  *   selected (nullable: every block) [requests][select_groups][budget]: logical
  *         ids, ascending and unique, selected_count [requests][select_groups]
- *         of them in use; KV heads share a list in groups of kv_heads /
+ *         of them in use (cut to 0 .. budget); KV heads share a list in groups of kv_heads /
  *         select_groups, as in the decode context. The block of the newest token is
  *         always attended and is not listed. Needs new_tokens = 1. An id that
  *         is out of range or not above the one before it is skipped and sets

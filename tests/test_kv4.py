@@ -888,3 +888,18 @@ def test_one_long_request_among_many_short_ones(pkg, cuda):
         want = torch.einsum("hgt,thd->hgd", torch.softmax(s, -1), v).reshape(4, d)
         # as in test_attention_batches: |v| up to 6, a logit summed from up to 60
         assert float((out[b].double() - want).abs().max()) <= 6 * (2.0 ** -20 * 60 + 2.0 ** -19)
+
+
+@pytest.mark.gpu
+def test_selected_counts_outside_the_list_are_cut(pkg, cuda):
+    """A count above the budget uses the whole list, one below zero none of it."""
+    rng = np.random.default_rng(45)
+    lens = [300, 300]
+    pool, table = _cache(rng, 2, lens, 1, 128, cuda)
+    q = _query(rng, (2, 4, 128), torch.float32, cuda)
+    selected = np.array([[[0, 4, 7]], [[1, 2, 3]]])
+    want = _check(pkg, q, pool, table, lens, cuda, selected=selected, counts=np.array([[3], [0]]))
+    out = pkg.attention_kv4(q, torch.as_tensor(pool, device=cuda), _i32(table, cuda), _i32(lens, cuda),
+                            selected=_i32(selected, cuda),
+                            selected_count=_i32([[(1 << 31) - 1], [-(1 << 31)]], cuda))
+    assert torch.equal(out, want)
