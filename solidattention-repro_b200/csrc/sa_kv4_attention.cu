@@ -28,10 +28,13 @@
 // small difference of large sums otherwise, and the matrix unit's truncating
 // sums lost 1e-4 of it at 4,128 tokens (9e-7 for plain FP32). FP32 queries
 // centre the key codes too, and add the products of their small parts apart.
-// Logits, maxima, sums and partial results are FP32. Value
-// steps are scaled by a power of two that follows their running maximum E, so
-// that weight * step stays inside FP16: steps 2^-24 below the largest one seen
-// by a warp vanish next to it.
+// Logits, maxima, sums and partial results are FP32. The value
+// steps of each group of 64 elements are scaled by a power of two 2^-E that
+// follows the group's largest finite one, so that weight * step stays inside
+// FP16. Groups are separate output elements: a huge or NaN step of one leaves
+// the others as they are. Inside a group, steps more than 2^-14 below the
+// largest one that a warp has seen lose bits (they are FP16 subnormals then,
+// off by 2^-25 of 2^E), an error of 2^-24 of the group's largest value.
 //
 // Work split. All (list, KV head, row tile) units' entries form one flat list;
 // every CTA takes an equal contiguous range of it, whatever the lengths, and
@@ -165,6 +168,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 // 2^k, -126 <= k <= 127.
 __device__ __forceinline__ float power_of_2(int k) { return __int_as_float((k + 127) << 23); }
+
+// k of a power of two 2^k held as FP16 bits in the low half (k up to 16, one above FP16's largest exponent).
+__device__ __forceinline__ int step_log2(uint32_t bits) { return static_cast<int>(bits >> 10 & 31u) - 15; }
 
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -530,9 +536,10 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
     float o[NT][NG][2][2][4];  // codes' sums of element 64 gr + 8 g + 4 w + 2 s (+ 1, times 16)
     float low[NT][2];          // minima's sums: lane group g holds value group g's
     float base[NT][2], sum[NT][2];  // running maximum - 11; sum of 2^(x - base)
-    int step_log2 = 0;              // E: value steps are held as s * 2^-E
-    uint32_t step_bits = 0;         // 2^E as FP16 bits, 0 before the first block
-    uint32_t step_unit = 0;         // 2^-E in both halves
+    uint32_t step_bits[NG];         // 2^E of each group as FP16 bits in both halves, 0 before the first block
+    uint32_t step_unit[NG];         // 2^-E in both halves: value steps are held as s * 2^-E
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) step_bits[gr] = step_unit[gr] = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -675,12 +682,14 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
       }
       // ---- running maxima of the logits and of the value steps, raised only
       // when a logit passes its row's by the headroom or a step passes 2^E
-      uint32_t most = 0;
+      uint32_t above = 0;  // bits 15 and 31: a step is not below its 2^E
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
-        most = __vimax3_u16x2(__vimax3_u16x2(step[gr][0][0], step[gr][0][1], step[gr][1][0]),
-                              step[gr][1][1], most);
-      bool passes = (most & 0xffffu) >= step_bits || most >> 16 >= step_bits;
+      for (int gr = 0; gr < NG; ++gr) {
+        const uint32_t most = __vmaxu2(__vimax3_u16x2(step[gr][0][0], step[gr][0][1], step[gr][1][0]),
+                                       step[gr][1][1]);
+        above |= (most | 0x80008000u) - step_bits[gr];  // 15-bit values: the halves do not borrow
+      }
+      bool passes = (above & 0x80008000u) != 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -709,26 +718,33 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
                 o[nt][gr][k >> 1][k & 1][c + 2] *= keep;
               }
           }
-        uint32_t largest = max(most & 0xffffu, most >> 16);
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        if (largest >= step_bits) {  // the same in every lane
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          // NaN and infinite steps (from 0x7c00 on) carry themselves through the products
+          uint32_t most = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w = step[gr][k >> 1][k & 1];
+            most = __vmaxu2(most, w & __vcmpltu2(w, 0x7c007c00u));
+          }
+          uint32_t largest = max(most & 0xffffu, most >> 16);
+          largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+          largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+          const uint32_t bits = step_bits[gr] & 0xffffu;
+          if (largest < bits) continue;  // the same in every lane
           // steps stay as they are while the largest is in [2^-8, 1)
           int exponent = static_cast<int>(largest >> 10) - 14;
           if (exponent > -8 && exponent <= 0) exponent = 0;
-          const float keep = step_bits == 0 ? 0.0f : power_of_2(step_log2 - exponent);
-          step_log2 = exponent;
-          step_bits = static_cast<uint32_t>(exponent + 15) << 10;
+          const float keep = bits == 0 ? 0.0f : power_of_2(step_log2(bits) - exponent);
+          step_bits[gr] = static_cast<uint32_t>(exponent + 15) * 0x04000400u;
           const __half2 unit = __half2half2(__float2half_rn(power_of_2(-exponent)));
-          step_unit = *reinterpret_cast<const uint32_t*>(&unit);
+          step_unit[gr] = *reinterpret_cast<const uint32_t*>(&unit);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) o[nt][gr][k >> 1][k & 1][c] *= keep;
+              for (int c = 0; c < 4; ++c) o[nt][gr][k >> 1][k & 1][c] *= keep;
         }
       }
       // ---- weights, as columns of the second product
@@ -758,7 +774,10 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
       if constexpr (kCentred) {
         // minimum + 8 step as an unevaluated sum of two FP16 numbers (Knuth's
         // two-sum), halved where 8 step could pass FP16's largest
-        const bool large = step_log2 > 12;
+        uint32_t bits = step_bits[0];
+#pragma unroll
+        for (int gr = 1; gr < NG; ++gr) bits = g == gr ? step_bits[gr] : bits;
+        const bool large = step_log2(bits) > 12;
         low_unit = large ? 2.0f : 1.0f;
         const uint32_t eight = large ? 0x44004400u : 0x48004800u, one = large ? 0x38003800u : 0x3c003c00u;
 #pragma unroll
@@ -817,7 +836,7 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t s = hmul2(step[gr][j][h], step_unit);
+            const uint32_t s = hmul2(step[gr][j][h], step_unit[gr]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               scaled[nt][0][j][h] = hmul2(weight[nt][0][j][h], s);
@@ -872,7 +891,6 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
     // ---- the segment's result
     const bool whole = count == n;
     const int part = ((static_cast<int>(blockIdx.x) * kWarps + warp) * 2 + (at == warp_begin ? 0 : 1)) * kTile;
-    const float code_unit = power_of_2((kCentred ? 0 : 24) + step_log2);
     const bool shared = joined && !whole;  // joined through shared memory
     float* mine = reinterpret_cast<float*>(ring);  // [kTile][kDim], then [kTile][2]
 #pragma unroll
@@ -888,6 +906,7 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           const float minima = __shfl_sync(0xffffffffu, low[nt][c], gr * 4 + t);
+          const float code_unit = power_of_2((kCentred ? 0 : 24) + step_log2(step_bits[gr]));
           float y[8];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {

@@ -1,0 +1,115 @@
+"""The 4-bit cache: what one value group, token or request holds stays out of the others.
+
+Bounds are held element by element: an output is measured against the values of its own
+group of 64 elements, so that a small group next to a huge one has to be right by itself.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_oracle as oracle4
+from test_kv4 import HALF_STEP, TYPES, _cache, _i32, _query
+
+BLOCK, GROUP = 32, 64
+
+
+def _value_places(d):
+    """Halfword indices in an entry of the value step and minimum of (row, group): each [32, d / 64]."""
+    _, _, _, _, step = oracle4.positions(d)
+    step = step[:, ::GROUP] // 2
+    return step, step + d // 2
+
+
+def _set_value(pool, table, d, b, token, head, group, step, minimum):
+    s, m = _value_places(d)
+    entry = pool.view(np.float16)[table[b, token // BLOCK], head]
+    entry[s[token % BLOCK, group]] = np.float16(step)
+    entry[m[token % BLOCK, group]] = np.float16(minimum)
+
+
+def _sizes(pool, table, lens, shape):
+    """The largest |step| 15 + |minimum| of an output element's group over the tokens its row sees: [B, T, QH, D]."""
+    n, new, qh, d = shape
+    kh = pool.shape[1]
+    size = np.zeros(shape)
+    for b in range(n):
+        blocks = -(-int(lens[b]) // BLOCK)
+        for h in range(kh if blocks else 0):
+            va = np.concatenate([oracle4.read_entry(pool[table[b, i], h])[3] for i in range(blocks)])
+            for i in range(new):
+                seen = va[:max(0, int(lens[b]) - new + i + 1)]
+                if len(seen):
+                    size[b, i, h * (qh // kh):(h + 1) * (qh // kh)] = np.nanmax(
+                        np.where(np.isfinite(seen), seen, 0.0), 0)
+    return size
+
+
+def _attend(pkg, q, pool, table, lens, device, **more):
+    return pkg.attention_kv4(q, torch.as_tensor(pool, device=device), _i32(table, device), _i32(lens, device), **more)
+
+
+def _check_elements(pkg, q, pool, table, lens, device):
+    """attention_kv4 against float64, element by element; not finite exactly where the formula is not.
+
+    A logit in FP32 is off by 2^-20 of the sum of its terms' sizes, which moves every weight by that much; weights,
+    sums and joins add 2^-19, and value steps held 2^-14 below their group's largest 2^-24, of the group's largest
+    value. BF16 outputs carry weights rounded to FP16 twice (2^-11 each). One rounding to the output type, whose
+    subnormals are 2^-25 off in FP16.
+    """
+    out = _attend(pkg, q, pool, table, lens, device)
+    q4 = q if q.dim() == 4 else q[:, None]
+    want, _, logit, _ = oracle4.attention(q4.double().cpu().numpy(), pool, table, lens, 1 / math.sqrt(q.shape[-1]))
+    got = out.double().cpu().numpy().reshape(want.shape)
+    size = _sizes(pool, table, lens, want.shape)
+    np.testing.assert_array_equal(np.isfinite(got), np.isfinite(want))
+    weight = 2.0 ** -20 * logit + 2.0 ** -19 + (2.0 ** -10 if out.dtype == torch.bfloat16 else 0.0)
+    tol = HALF_STEP[out.dtype] * np.abs(want) * (1 + 2.0 ** -7) + weight[..., None] * size + 2.0 ** -25
+    finite = np.isfinite(want)
+    off = np.abs(got[finite] - want[finite]) / tol[finite]
+    assert off.max() <= 1, f"{off.max():.3g} of the tolerance"
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("small", [1.0, 0.06])
+@pytest.mark.parametrize("step, minimum", [(np.nan, np.nan), (np.inf, 0.0), (8736.0, -65504.0), (300.0, -2000.0),
+                                           (0.0, 3.0), (2.0 ** -24, 2.0 ** -24)])
+def test_a_group_of_another_size_leaves_the_others_as_they_are(pkg, cuda, dtype, d, small, step, minimum):
+    """One token, then every token, with an extreme group 0; the other groups at 0.3 and 0.02 a step."""
+    rng = np.random.default_rng(d)
+    lens = [700, 45, 33]
+    pool, table = _cache(rng, 3, lens, 2, d, cuda, scale=small)
+    q = _query(rng, (3, 8, d), dtype, cuda)
+    for tokens in ([3], range(700)):
+        for token in tokens:
+            for head in range(2):
+                _set_value(pool, table, d, 0, token, head, 0, step, minimum)
+        _check_elements(pkg, q, pool, table, lens, cuda)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 65504.0, -1e4])
+def test_an_extreme_element_reaches_its_own_group_alone(pkg, cuda, dtype, value):
+    """Through pack_kv4: one element of one token's values, and the outputs of all other groups."""
+    rng = np.random.default_rng(7)
+    kh, d, tokens = 2, 128, 300
+    k, v = (torch.from_numpy(rng.standard_normal((tokens, kh, d))).to(dtype).to(cuda) for _ in range(2))
+    v = v * 0.03
+    v[20, 1, 70] = value
+    pool = pkg.kv4_pool(10, kh, d, device=cuda)
+    pkg.pack_kv4(pool, k, v, torch.arange(tokens, dtype=torch.int32, device=cuda))
+    table = np.arange(10)[None]
+    q = _query(rng, (1, 8, d), dtype, cuda)
+    out = _check_elements(pkg, q, pool.cpu().numpy(), table, [tokens], cuda)
+    clean = pool.clone()
+    v[20, 1, 70] = 0
+    pkg.pack_kv4(clean, k, v, torch.arange(tokens, dtype=torch.int32, device=cuda))
+    was = _check_elements(pkg, q, clean.cpu().numpy(), table, [tokens], cuda)
+    assert torch.equal(out[0, :4], was[0, :4]) and torch.equal(out[0, 4:, :64], was[0, 4:, :64])
