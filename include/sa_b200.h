@@ -255,7 +255,9 @@ SA_API sa_status sa_unpack_kv4(const void* pool, size_t pool_blocks,
  *   block_table [requests][table_blocks]; seq_lens [requests]: tokens held, the
  *         new ones included. Query i of request b stands at position
  *         seq_lens[b] - new_tokens + i and sees positions up to its own; one
- *         that sees none gives zeros (and -inf in lse_out).
+ *         that sees none gives zeros (and -inf in lse_out). What stands behind
+ *         its position, NaN too, does not reach it; a NaN value group that it
+ *         sees makes that group of its output NaN, a NaN key group the row.
  *   selected (nullable: every block) [requests][select_groups][budget]: logical
  *         ids, ascending and unique, selected_count [requests][select_groups]
  *         of them in use (cut to 0 .. budget); KV heads share a list in groups of kv_heads /

@@ -532,6 +532,8 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
       }
     }
     const int least = length - p.new_tokens + 1 + row0 / p.group;  // what every row sees
+    // what the last row sees
+    const int longest = length - p.new_tokens + 1 + (min(row0 + kTile, p.rows) - 1) / p.group;
 
     float o[NT][NG][2][2][4];  // codes' sums of element 64 gr + 8 g + 4 w + 2 s (+ 1, times 16)
     float low[NT][2];          // minima's sums: lane group g holds value group g's
@@ -557,10 +559,19 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
           for (int c = 0; c < 4; ++c) o[nt][gr][m >> 1][m & 1][c] = 0.0f;
     }
 
-    // One entry: the block whose first token is token0, `held` of its rows in
-    // use. Blocks that every row sees whole take the copy without masks.
-    auto process = [&](const uint8_t* entry, int token0, int held, auto masks) {
+    // One entry. Blocks that every row sees whole take the copy without masks.
+    // Of the block whose first token is token0, the other one takes the rows
+    // that see at least `from` and at most `to` of its tokens.
+    auto process = [&](const uint8_t* entry, int token0, int from, int to, auto masks) {
       constexpr bool kMasked = decltype(masks)::value;
+      bool sees[NT][2];  // columns 2t, 2t + 1 take part
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int held = min(limit[nt][c] - token0, kBlockTokens);
+          sees[nt][c] = !kMasked || (held >= from && held <= to);
+        }
       // ---- logits
       float x[NT][2][4];
       uint4 scales[NG];  // (step, minimum) of rows g, g + 8, g + 16, g + 24
@@ -645,7 +656,7 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-              if (token0 + 16 * j + 8 * (c >> 1) + g >= limit[nt][c & 1])
+              if (!sees[nt][c & 1] || token0 + 16 * j + 8 * (c >> 1) + g >= limit[nt][c & 1])
                 x[nt][j][c] = -INFINITY;
       }
 
@@ -668,13 +679,13 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
         minimum[1][0] = w.z;
         minimum[1][1] = w.w;
       }
-      if constexpr (kMasked) {  // rows that are not held: nothing of them may enter a product
+      if constexpr (kMasked) {  // tokens that no row sees: nothing of them may enter a product
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = 16 * j + 8 * h + 2 * t;
-            const uint32_t keep = (r < held ? 0xffffu : 0u) | (r + 1 < held ? 0xffff0000u : 0u);
+            const uint32_t keep = (r < to ? 0xffffu : 0u) | (r + 1 < to ? 0xffff0000u : 0u);
             minimum[j][h] &= keep;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) step[gr][j][h] &= keep;
@@ -802,8 +813,10 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
           for (int part = 0; part < kWeights; ++part)
             mma16816(acc, minimum[j][0], rest[j][0], minimum[j][1], rest[j][1],
                      weight[nt][part][j][0], weight[nt][part][j][1]);
-        low[nt][0] = kCentred ? fmaf(acc[0] + acc[2], low_unit, low[nt][0]) : low[nt][0] + acc[0];
-        low[nt][1] = kCentred ? fmaf(acc[1] + acc[3], low_unit, low[nt][1]) : low[nt][1] + acc[1];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (sees[nt][c])
+            low[nt][c] = kCentred ? fmaf(acc[c] + acc[c + 2], low_unit, low[nt][c]) : low[nt][c] + acc[c];
       }
       // ---- weighted codes
       uint32_t word[2][2][2 * NG];
@@ -864,27 +877,56 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
                            scaled[nt][part][j][0], scaled[nt][part][j][1]);
               }
 #pragma unroll
-              for (int c = 0; c < 4; ++c) o[nt][gr][w][s][c] += acc[c];
+              for (int c = 0; c < 4; ++c)
+                if (sees[nt][c & 1]) o[nt][gr][w][s][c] += acc[c];
             }
       }
     };
 
-    int stage = 0;
-    for (int i = 0; i < count; ++i) {
-      cp_async_wait<kStages - 1>();
-      __syncwarp();
+    // A token that some rows see and others do not has a weight of zero for
+    // these, which leaves them as they are unless its values are not finite (zero
+    // times that is NaN) or its steps raise their group's exponent. Does one of
+    // an entry's tokens from .. to - 1 forbid to take such rows together? (Always
+    // apart, 16 requests with 4 drafts each took 171 us instead of 150.)
+    auto parts_rows = [&](const uint8_t* entry, int from, int to) {
+      bool parts = false;
+      if (lane >= from && lane < to) {
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const auto* at = reinterpret_cast<const uint16_t*>(entry + kv4_value_scale_at(kDim, lane, gr));
+          parts |= at[0] >= (step_bits[gr] & 0xffffu) || (at[kDim / 2] & 0x7c00u) == 0x7c00u;
+        }
+      }
+      return __any_sync(0xffffffffu, parts);
+    };
+
+    int stage = 0, seen = 0;  // seen: tokens of a masked block that its last turn's rows saw
+    for (int i = 0; i < count;) {
+      if (seen == 0) {
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+      }
       if (!(unread >> stage & 1)) {
         const uint8_t* entry = ring + stage * kStage;
         const int logical = ids ? newest : first + i;  // with ids, used for the newest block only
         const int token0 = logical * kBlockTokens;
-        if ((!ids || first + i == n - 1) && token0 + kBlockTokens > least)
-          process(entry, token0, min(length - token0, kBlockTokens), std::true_type{});
-        else
-          process(entry, token0, kBlockTokens, std::false_type{});
+        if ((!ids || first + i == n - 1) && token0 + kBlockTokens > least) {
+          const int from = max(least - token0, seen + 1), most = min(longest - token0, kBlockTokens);
+          seen = most;
+          if (from <= most) {
+            if (from < most && parts_rows(entry, from, most)) seen = from;
+            process(entry, token0, from, seen, std::true_type{});
+          }
+          if (seen < most) continue;
+        } else {
+          process(entry, token0, 0, kBlockTokens, std::false_type{});
+        }
       }
+      seen = 0;
       __syncwarp();  // every lane has read the stage
       fetch(i + kStages, stage);
       stage = stage + 1 == kStages ? 0 : stage + 1;
+      ++i;
     }
     cp_async_wait<0>();
 

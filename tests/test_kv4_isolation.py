@@ -113,3 +113,48 @@ def test_an_extreme_element_reaches_its_own_group_alone(pkg, cuda, dtype, value)
     pkg.pack_kv4(clean, k, v, torch.arange(tokens, dtype=torch.int32, device=cuda))
     was = _check_elements(pkg, q, clean.cpu().numpy(), table, [tokens], cuda)
     assert torch.equal(out[0, :4], was[0, :4]) and torch.equal(out[0, 4:, :64], was[0, 4:, :64])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group, d", [(1, 64), (3, 128), (4, 128), (2, 256)])
+@pytest.mark.parametrize("new", [2, 5, 9, 40])
+@pytest.mark.parametrize("step, minimum", [(np.nan, np.nan), (np.inf, -np.inf), (8736.0, -65504.0)])
+def test_a_later_token_does_not_reach_earlier_rows(pkg, cuda, dtype, group, d, new, step, minimum):
+    """Extreme values and NaN keys in the newest tokens: the rows before them keep their bytes."""
+    rng = np.random.default_rng(new * 100 + d)
+    lens = [64 + new // 2, 32 + new, 700, new]  # new tokens across a block's end, from its first row, far on, alone
+    pool, table = _cache(rng, 4, lens, 2, d, cuda)
+    q = _query(rng, (4, new, 2 * group, d), dtype, cuda)
+    clean = _check_elements(pkg, q, pool, table, lens, cuda)
+    _, _, _, key_step, _ = oracle4.positions(d)
+    for behind in sorted({1, new // 2, new - 1}):  # the last, a middle and the second token
+        dirty = pool.copy()
+        for b, length in enumerate(lens):
+            token = length - behind
+            for head in range(2):
+                _set_value(dirty, table, d, b, token, head, 0, step, minimum)
+                if d > 64:
+                    _set_value(dirty, table, d, b, token, head, 1, -step, minimum)
+            dirty.view(np.float16)[table[b, token // BLOCK], 1, key_step[token % BLOCK, 0] // 2] = np.nan
+        out = _attend(pkg, q, dirty, table, lens, cuda)
+        assert torch.equal(out[:, :new - behind], clean[:, :new - behind])
+        assert out[:, new - behind:, group:].isnan().all()  # the second KV head's keys
+        if not math.isfinite(step):
+            assert not out[:, new - behind:, :, :64].isfinite().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new, group, longest", [(3, 4, 5000), (8, 1, 900), (6, 8, 300)])
+def test_rows_see_their_own_tokens_with_every_element_bounded(pkg, cuda, dtype, new, group, longest):
+    """Values that grow along the request: a row that saw one token more or less would be far off."""
+    rng = np.random.default_rng(longest)
+    lens = [int(x) for x in rng.integers(new, longest, 5)] + [longest, 31 + new, 1]
+    pool, table = _cache(rng, len(lens), lens, 2, 128, cuda)
+    for b, length in enumerate(lens):
+        for k in range(min(new, length)):
+            for head in range(2):
+                for g in range(2):
+                    _set_value(pool, table, 128, b, length - 1 - k, head, g, 2.0 ** (new - k - 3), 4.0 ** (new - k))
+    _check_elements(pkg, _query(rng, (len(lens), new, 2 * group, 128), dtype, cuda), pool, table, lens, cuda)
