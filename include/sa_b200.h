@@ -209,11 +209,12 @@ SA_API size_t sa_kv4_entry_bytes(size_t head_dim);
  * those given back are pushed after that in reverse order, so that a step
  * followed by its inverse restores the list. A request whose growth does not
  * fit is refused: its length, blocks and table row stay, its tokens get slot
- * -1, and a status bit is set: SA_DEV_TABLE_FULL (the table's row is too
- * short), SA_DEV_SLOTS_FULL (its last row is beyond max_tokens, be it only by
- * the tokens of requests before it),
- * SA_DEV_POOL_EMPTY (the blocks that it and the requests before it need exceed
- * the free ones). SA_DEV_BAD_BLOCK: a length, table entry or list entry was
+ * -1 and keep their rows, and a status bit is set: SA_DEV_TABLE_FULL (the
+ * table's row is too short), SA_DEV_SLOTS_FULL (its last row is beyond
+ * max_tokens, be it only by the tokens of requests before it, refused ones
+ * included), SA_DEV_POOL_EMPTY (the blocks that it and the requests before it need exceed
+ * the free ones). A request that does not grow is never refused for want of
+ * room. SA_DEV_BAD_BLOCK: a length, table entry or list entry was
  * outside its range. requests <= 8192. */
 SA_API sa_status sa_plan_blocks(const int32_t* add, size_t requests,
                                 int32_t* seq_lens, int32_t* block_table,

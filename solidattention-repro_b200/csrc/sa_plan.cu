@@ -159,7 +159,9 @@ __device__ __forceinline__ Request request_of(const PlanParams& p, int b, uint32
   r.grow = max(add, 0);
   r.full = !r.broken && after > limit;
   const uint32_t room = max(p.max_tokens - static_cast<int>(tok_at), 0);
-  r.over = add_capped(tok_at, r.grow) > static_cast<uint32_t>(p.max_tokens);
+  // only what grows needs rows: requests that end or shrink behind a prompt too
+  // long for the slot map give their blocks back all the same
+  r.over = r.grow > 0 && add_capped(tok_at, r.grow) > static_cast<uint32_t>(p.max_tokens);
   r.rows = static_cast<int>(min(static_cast<uint32_t>(r.grow), room));
   r.held = blocks_of(r.before);
   r.want = r.refused() ? r.held : blocks_of(static_cast<int>(after));

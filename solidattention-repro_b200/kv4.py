@@ -105,9 +105,9 @@ def plan_blocks(add: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Te
     [pool blocks] and ``free_top`` [1] (int32) are the state, changed in place.
     Returns (slots [max_tokens], positions [max_tokens], cu_tokens [requests +
     1]): the slots and positions of the new tokens request by request, -1 and 0
-    behind the last, and each request's first row. A request that does not fit
-    is left as it was, its slots are -1 and a status bit is set
-    (sa_plan_blocks).
+    behind the last, and each request's first row. A request whose growth does
+    not fit is left as it was, its slots are -1 and a status bit is set; those
+    that shrink or end always do (sa_plan_blocks).
     """
     ptr = _tensor(add, torch.int32, 1, "add")
     dev = add.get_device()

@@ -88,7 +88,7 @@ def plan(add, lens, table, free, top, max_tokens):
         grow = max(int(add[b]), 0)
         after = max(int(lens[b]) + int(add[b]), 0)
         held, want = -(-int(lens[b]) // BLOCK), -(-after // BLOCK)
-        why = "table" if want > width else "slots" if cu[-1] + grow > max_tokens else None
+        why = "table" if want > width else "slots" if grow and cu[-1] + grow > max_tokens else None
         if why is None:
             need = max(want - held, 0)
             wanted += need
