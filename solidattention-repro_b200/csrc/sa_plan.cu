@@ -268,8 +268,9 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
   else
     __syncthreads();
 
-  for (int r = me; r < given; r += all) {
-    const int b = owner_of(give, n, r);
+  // up to 2^31 - 1 where lengths claim more blocks than the pool has: r + all passes 31 bits
+  for (uint32_t r = me; r < static_cast<uint32_t>(given); r += all) {
+    const int b = owner_of(give, n, static_cast<int>(r));
     const int before = len[b] & 0x7fffffff;
     const int after = max(before + p.add[b], 0);  // gives back, so add < 0 and not refused
     const int id = p.table[static_cast<int64_t>(b) * p.table_blocks + blocks_of(after) + r - give[b]];

@@ -44,3 +44,32 @@ def test_requests_that_do_not_grow_are_served_behind_refused_prompts(pkg, cuda, 
     for b in range(1, n):
         assert (refused[b] == "slots") == (add[b] > 0)
     np.testing.assert_array_equal(state.lens[1:], np.where(add > 0, before, np.maximum(before + add, 0))[1:])
+
+
+def test_loop_over_given_blocks_ends_in_unsigned_arithmetic():
+    """The largest table of the documented limits: a signed index would wrap below zero behind its last block."""
+    requests, width, threads = 8192, (1 << 31) // 8192 - 1, 16 * 1024
+    given = requests * width  # every request gives every block of its row back
+    assert given <= (1 << 31) - 1
+    last = given - 1 - (given - 1) % threads  # the last turn's first index
+    with np.errstate(over="ignore"):
+        signed = np.int32(last) + np.int32(threads)
+        unsigned = np.uint32(last) + np.uint32(threads)
+    assert signed < 0 and unsigned >= given
+
+
+@pytest.mark.gpu
+def test_a_full_table_of_the_largest_size_given_back(pkg, cuda):
+    """8,192 requests of 262,143 blocks each, far more than the pool: flagged, the list full, nothing out of range."""
+    n, width, pool = 8192, (1 << 31) // 8192 - 1, 64
+    table = torch.zeros(n, width, dtype=torch.int32, device=cuda)
+    table[-1] = 7
+    lens = torch.full((n,), width * 32, dtype=torch.int32, device=cuda)
+    add = torch.full((n,), -(1 << 31), dtype=torch.int32, device=cuda)
+    free, top = _i32(np.full(pool, 5), cuda), _i32([10], cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    slots, positions, cu = pkg.plan_blocks(add, lens, table, free, top, 3, status=status)
+    assert int(status) == pkg.SA_DEV_BAD_BLOCK and int(top) == pool
+    assert not lens.any() and not cu.any() and (slots == -1).all() and not positions.any()
+    # the last blocks given back are the first above the old top: those of the last request
+    assert free.tolist() == [5] * 10 + [7] * (pool - 10)
