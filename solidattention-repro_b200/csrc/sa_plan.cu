@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
   int32_t* len = give + n;        // [n] its length before, bit 31 set when refused
   int32_t* chunk = len + n;       // [n] first of its chunks of kChunk tokens
   if (threadIdx.x == 0) taken_shared = 0;
+  if (n <= 32) __syncthreads();  // before any warp's maximum; for more requests the scans have barriers
 
   int top = *p.free_top;
   if (top < 0 || top > p.pool_blocks) {
