@@ -33,7 +33,9 @@ constexpr int kPlanMaxRequests = 8192;
 constexpr int kPlanArrays = 5;  // of one int a request in shared memory
 constexpr int kFew = 4;         // new tokens that a request's own thread writes
 constexpr int kChunk = 128;     // new tokens that a warp writes at a time otherwise
-constexpr int kPlanCluster = 16;  // the largest; 8 took 22 us where 16 took 18 (2,000 requests, 156,200 rows)
+// The largest cluster. 2,000 requests, 156,200 rows of slots: 14.2 us a plan with 16 CTAs, 18.9 with 8, 42 with
+// 2, 71 with one.
+constexpr int kPlanCluster = 16;
 
 struct PlanParams {
   const int32_t* add;
@@ -294,11 +296,49 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanParams p) {
 }
 
 int g_plan_smem[kMaxDevices];
-bool g_plan_wide[kMaxDevices];  // clusters above the portable size allowed
+// Cluster size for up to kPlanHalf bytes of shared memory a CTA (two may share an SM), and above; 0: not yet asked.
+constexpr int kPlanHalf = 100 * 1024, kPlanMost = kPlanMaxRequests * kPlanArrays * (int)sizeof(int32_t);
+int g_plan_cluster[kMaxDevices][2];
 
 int plan_device() {
   int device = 0;
   return cudaGetDevice(&device) == cudaSuccess && device >= 0 && device < kMaxDevices ? device : 0;
+}
+
+cudaLaunchConfig_t plan_config(cudaLaunchAttribute* attr, int ctas, int threads, int bytes) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = bytes;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = ctas;
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  return cfg;
+}
+
+// CTAs of a large step: the largest cluster that the current device can place (one on a share of a GPU
+// without so many SMs side by side). The kernel takes any size.
+sa_status plan_cluster(int bytes, int* ctas) {
+  const int wide = bytes > kPlanHalf;
+  int& known = g_plan_cluster[plan_device()][wide];
+  if (known == 0) {
+    SA_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel),
+                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    int size = kPlanCluster;
+    for (; size > 1; size /= 2) {
+      cudaLaunchAttribute attr;
+      const cudaLaunchConfig_t cfg = plan_config(&attr, size, 1024, wide ? kPlanMost : kPlanHalf);
+      int active = 0;
+      if (cudaOccupancyMaxActiveClusters(&active, plan_kernel, &cfg) == cudaSuccess && active > 0) break;
+      cudaGetLastError();  // a size that cannot be asked for is one that does not fit
+    }
+    known = size;
+  }
+  *ctas = known;
+  return SA_OK;
 }
 
 }  // namespace
@@ -327,30 +367,20 @@ extern "C" SA_API sa_status sa_plan_blocks(const int32_t* add, size_t requests, 
   PlanParams p{add,       seq_lens,  block_table,   free_list, free_top,
                slots_out, positions_out, cu_tokens_out, status,    (int)requests,
                (int)table_blocks, (int)pool_blocks, (int)max_tokens};
-  // One CTA up to 4096 tokens and 1024 requests, else a cluster of 16.
+  // One CTA up to 4096 tokens and 1024 requests, else one cluster.
   const bool small = max_tokens <= 4096 && requests <= 1024;
   const int threads = small && requests <= 256 && max_tokens <= 1024 ? 256 : 1024;
   const int bytes = (int)requests * kPlanArrays * (int)sizeof(int32_t);
   const sa_status st =
-      ensure_smem_limit(reinterpret_cast<const void*>(plan_kernel),
-                        kPlanMaxRequests * kPlanArrays * (int)sizeof(int32_t), g_plan_smem);
+      ensure_smem_limit(reinterpret_cast<const void*>(plan_kernel), kPlanMost, g_plan_smem);
   if (st != SA_OK) return st;
-  if (!small && !g_plan_wide[plan_device()]) {
-    SA_CUDA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(plan_kernel),
-                                     cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    g_plan_wide[plan_device()] = true;
+  int ctas = 1;
+  if (!small) {
+    const sa_status placed = plan_cluster(bytes, &ctas);
+    if (placed != SA_OK) return placed;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(small ? 1 : kPlanCluster);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = bytes;
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = plan_config(&attr, ctas, threads, bytes);
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cfg.gridDim.x;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = small ? 0 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, plan_kernel, p), "plan launch");
 }
