@@ -189,7 +189,9 @@ SA_API sa_status sa_pack_kv_fp16(uint16_t* packed, const float* key,
  *   the value held is s * c + m: within s / 2 of x.
  *
  * Finite elements are first clamped to +-65504; a NaN or infinite element
- * makes its whole group NaN. head_dim is 64, 128 or 256. */
+ * makes its whole group NaN. Next to the range's end s * 15 + m may pass 65504
+ * (by up to 112), since s is rounded up; FP16 outputs stop at 65504.
+ * head_dim is 64, 128 or 256. */
 SA_API size_t sa_kv4_entry_bytes(size_t head_dim);
 
 /* Bring a batch's block tables, lengths and free list from one step to the

@@ -98,18 +98,6 @@ __device__ __forceinline__ int64_t entry_of(int slot, int kv_heads, int head) {
   return (static_cast<int64_t>(slot / kBlockTokens) * kv_heads + head) * kv4_entry_bytes(64 * NG);
 }
 
-// Minimum and maximum that are NaN if an operand is.
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float c;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-  return c;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float c;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-  return c;
-}
-
 // Sixteen elements as they are loaded: 16-bit types stay packed until their
 // minimum and maximum are known.
 template <int TYPE>
@@ -353,6 +341,11 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const UnpackParams p) 
         y[8 * k + e] = Element::store(fmaf(s, code.x, m));  // the product is exact: one rounding
         y[8 * k + e + 4] = Element::store(fmaf(s, code.y, m));
       }
+    if constexpr (TYPE == SA_TYPE_F16) {
+      __half2* pairs = reinterpret_cast<__half2*>(y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) pairs[k] = __hmin2_nan(pairs[k], __float2half2_rn(kHalfMost));
+    }
     // Two lanes exchange quads, so that each store of the warp writes whole
     // 32-byte sectors.
     uint4* to = reinterpret_cast<uint4*>(row + static_cast<int64_t>(i) * p.kv_heads * kDim);

@@ -57,6 +57,23 @@ __device__ __forceinline__ int kv4_value_scale_at(int d, int r, int group) {
   return kv4_value_scales(d) + 64 * group + 2 * order;
 }
 
+// Minimum and maximum that are NaN if an operand is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float c;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
+
+// The largest FP16 number, where FP16 outputs stop (NaN stays). The step is rounded up, so
+// the code 15 of a row next to the range's end stands for up to 65,616, which would be
+// infinite in FP16. Held values are not below the minimum, so not below -65,504.
+constexpr float kHalfMost = 65504.0f;
+
 // ---- element types of the calls (SA_TYPE_*) -------------------------------------
 
 template <int TYPE>

@@ -107,6 +107,11 @@ __device__ __forceinline__ uint32_t pack_bf162(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Outputs in FP16: finite ones stay so.
+__device__ __forceinline__ uint32_t pack_output(float a, float b) {
+  return pack_half2(min_nan(a, kHalfMost), min_nan(b, kHalfMost));
+}
+
 // Eight consecutive elements from element `i` on (a multiple of 8).
 __device__ __forceinline__ void store8(void* base, int64_t i, int type, const float (&x)[8]) {
   if (type == SA_TYPE_F32) {
@@ -115,8 +120,8 @@ __device__ __forceinline__ void store8(void* base, int64_t i, int type, const fl
     at[1] = make_float4(x[4], x[5], x[6], x[7]);
   } else if (type == SA_TYPE_F16) {
     *reinterpret_cast<uint4*>(static_cast<__half*>(base) + i) =
-        make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]),
-                   pack_half2(x[6], x[7]));
+        make_uint4(pack_output(x[0], x[1]), pack_output(x[2], x[3]), pack_output(x[4], x[5]),
+                   pack_output(x[6], x[7]));
   } else {
     *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + i) =
         make_uint4(pack_bf162(x[0], x[1]), pack_bf162(x[2], x[3]), pack_bf162(x[4], x[5]),
@@ -131,7 +136,7 @@ __device__ __forceinline__ void store4(void* base, int64_t i, int type, float a,
     *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = make_float4(a, b, c, d);
   else if (type == SA_TYPE_F16)
     *reinterpret_cast<uint2*>(static_cast<__half*>(base) + i) =
-        make_uint2(pack_half2(a, b), pack_half2(c, d));
+        make_uint2(pack_output(a, b), pack_output(c, d));
   else
     *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(base) + i) =
         make_uint2(pack_bf162(a, b), pack_bf162(c, d));
@@ -1097,7 +1102,7 @@ __device__ __forceinline__ void store1(void* base, int64_t i, int type, float x)
   if (type == SA_TYPE_F32)
     static_cast<float*>(base)[i] = x;
   else if (type == SA_TYPE_F16)
-    static_cast<__half*>(base)[i] = __float2half_rn(x);
+    static_cast<__half*>(base)[i] = __float2half_rn(min_nan(x, kHalfMost));
   else
     static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
 }

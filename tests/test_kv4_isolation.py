@@ -158,3 +158,53 @@ def test_rows_see_their_own_tokens_with_every_element_bounded(pkg, cuda, dtype, 
                 for g in range(2):
                     _set_value(pool, table, 128, b, length - 1 - k, head, g, 2.0 ** (new - k - 3), 4.0 ** (new - k))
     _check_elements(pkg, _query(rng, (len(lens), new, 2 * group, 128), dtype, cuda), pool, table, lens, cuda)
+
+
+def _at_the_end_of_the_range(cuda, d=128):
+    """Rows [6, 1, d] whose held values pass FP16's range: the step is rounded up."""
+    x = torch.zeros(6, 1, d, device=cuda)
+    x[0, 0, ::2], x[0, 0, 1::2] = 65504.0, -65504.0  # 65,536 at code 15
+    x[1, 0, ::2] = 65504.0                            # 65,520: the smallest that FP16 rounds to infinity
+    x[2, 0] = torch.linspace(-65504.0, 65504.0, d, device=cuda)
+    x[3, 0] = torch.linspace(60000.0, 65504.0, d, device=cuda)
+    x[4, 0, ::2], x[4, 0, 1::2] = 1e30, -1e30         # clamped first
+    x[5, 0, 3] = float("inf")                         # its group is NaN, whatever the type
+    return x
+
+
+@pytest.mark.gpu
+def test_finite_rows_stay_finite_in_every_type(pkg, cuda):
+    x = _at_the_end_of_the_range(cuda)
+    pool = pkg.kv4_pool(1, 1, 128, device=cuda)
+    slots = torch.arange(6, dtype=torch.int32, device=cuda)
+    pkg.pack_kv4(pool, x, -x, slots)
+    held = pkg.unpack_kv4(pool, slots, torch.float32)
+    assert float(held[0][:5].max()) > 65519 and held[0][5, 0, :64].isnan().all()
+    for got, want in zip(pkg.unpack_kv4(pool, slots, torch.float16), held):
+        assert torch.equal(got.isnan(), want.isnan())
+        want = want.clamp(-65504.0, 65504.0)
+        off = (got.double() - want.double()).abs().nan_to_num(0.0)
+        assert (off <= (want.double().abs() * 2.0 ** -11).nan_to_num(0.0) + 2.0 ** -25).all()
+    for got, want in zip(pkg.unpack_kv4(pool, slots, torch.bfloat16), held):
+        assert torch.equal(got.isfinite(), want.isfinite())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("query, out", [(torch.float16, None), (torch.float32, torch.float16),
+                                        (torch.bfloat16, None), (torch.float32, None)])
+@pytest.mark.parametrize("tokens", [1, 40, 4000])
+def test_attention_over_finite_rows_is_finite(pkg, cuda, query, out, tokens):
+    """All tokens hold the same extreme row: written at once, joined in a CTA, and joined from many parts."""
+    x = _at_the_end_of_the_range(cuda)[1:2].expand(tokens, 1, 128)
+    pool = pkg.kv4_pool(tokens // 32 + 1, 1, 128, device=cuda)
+    pkg.pack_kv4(pool, x * 0, x, torch.arange(tokens, dtype=torch.int32, device=cuda))
+    table = np.arange(tokens // 32 + 1)[None]
+    got = _attend(pkg, torch.ones(1, 4, 128, dtype=query, device=cuda), pool.cpu().numpy(), table, [tokens], cuda,
+                  out_dtype=out)
+    want = oracle4.values(x[0, 0].double().cpu().numpy())
+    if got.dtype == torch.float16:
+        want = want.clip(-65504, 65504)
+    assert got.isfinite().all()
+    # the sum of equal values: FP32 sums (2^-19) and one rounding; BF16 weights as above
+    tol = np.abs(want) * (HALF_STEP[got.dtype] + 2.0 ** -19 + (2.0 ** -10 if got.dtype == torch.bfloat16 else 0)) + 0.1
+    assert (np.abs(got.double().cpu().numpy() - want) <= tol).all()
