@@ -107,7 +107,8 @@ def plan_blocks(add: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Te
     1]): the slots and positions of the new tokens request by request, -1 and 0
     behind the last, and each request's first row. A request whose growth does
     not fit is left as it was, its slots are -1 and a status bit is set; those
-    that shrink or end always do (sa_plan_blocks).
+    that shrink or end always do (sa_plan_blocks). A batch without requests is
+    an empty plan.
     """
     ptr = _tensor(add, torch.int32, 1, "add")
     dev = add.get_device()
@@ -120,6 +121,9 @@ def plan_blocks(add: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Te
         raise ValueError("add, seq_lens and block_table must have a row a request, free_top one element")
     if max_tokens < 0:
         raise ValueError("max_tokens must not be negative")
+    if n == 0:  # an idle batch
+        _status(status, dev)
+        return add.new_full((max_tokens,), -1), add.new_zeros(max_tokens), add.new_zeros(1)
     slots, positions, cu = add.new_empty(max_tokens), add.new_empty(max_tokens), add.new_empty(n + 1)
     _call(dev, "plan_blocks", load().sa_plan_blocks, ptr, n, lens, table, block_table.shape[1], free,
           free_list.shape[0], top, max_tokens, slots.data_ptr(), positions.data_ptr(), cu.data_ptr(),
@@ -217,6 +221,12 @@ def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Te
     lse = query.new_empty(shape[:-1], dtype=torch.float32) if return_lse else None
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    if n == 0:  # an idle batch
+        _status(status, dev)
+        return (out, lse) if return_lse else out
+    if block_table.shape[1] == 0:  # no request holds a block: a column without one stands for it
+        block_table = block_table.new_full((n, 1), -1)
+        table = block_table.data_ptr()
     ws_bytes = _workspace_bytes(n, new, qh, heads, d, dev)
     ws = pool.new_empty(ws_bytes or 16)
     _call(dev, "attention_kv4", lib.sa_attention_kv4, q, _TYPES[query.dtype], query.stride(0),
