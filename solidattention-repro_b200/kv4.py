@@ -189,12 +189,15 @@ def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Te
     logical blocks (ascending; as from select_shared_blocks) and the block of
     the newest token. Returns the output in the query's shape and type
     (``out_dtype`` for a float32 query), and with ``return_lse`` also the
-    log-sum-exp of the logits, FP32, without head_dim (sa_attention_kv4).
+    log-sum-exp of the logits, FP32, without head_dim (sa_attention_kv4). There
+    is no backward pass: a query that requires grad is refused in grad mode.
     """
     ptr, blocks, heads, d = _pool_dims(pool)
     dev = pool.get_device()
     lead = 4 if isinstance(query, torch.Tensor) and query.dim() == 4 else 3
     q = _rows(query, lead, "query", dev)
+    if query.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("attention_kv4 has no backward pass: call it under torch.no_grad() or detach the query")
     n, qh = query.shape[0], query.shape[-2]
     new = query.shape[1] if lead == 4 else 1
     table = _tensor(block_table, torch.int32, 2, "block_table", dev)

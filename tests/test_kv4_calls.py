@@ -1,10 +1,11 @@
-"""Calls of the 4-bit cache that a serving loop makes at its edges: no requests, no blocks."""
+"""Calls of the 4-bit cache that a serving loop makes at its edges: no requests, no blocks, grad mode."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
-from test_kv4 import _i32
+from test_kv4 import _cache, _i32, _query
 
 
 @pytest.mark.gpu
@@ -40,3 +41,20 @@ def test_a_table_without_columns_holds_nothing(pkg, cuda):
     assert not out.any() and torch.isneginf(lse).all() and int(status) == 0
     out = pkg.attention_kv4(q, pool, table, _i32([0, 5, 50], cuda), status=status)
     assert not out.any() and int(status) == pkg.SA_DEV_BAD_BLOCK
+
+
+@pytest.mark.gpu
+def test_a_query_that_requires_grad_is_refused_in_grad_mode(pkg, cuda):
+    rng = np.random.default_rng(1)
+    pool, table = _cache(rng, 1, [40], 2, 128, cuda)
+    args = [torch.as_tensor(pool, device=cuda), _i32(table, cuda), _i32([40], cuda)]
+    q = _query(rng, (1, 4, 128), torch.float32, cuda)
+    want = pkg.attention_kv4(q, *args)
+    q.requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        pkg.attention_kv4(q, *args)
+    with torch.no_grad():
+        assert torch.equal(pkg.attention_kv4(q, *args), want)
+    with torch.inference_mode():
+        assert torch.equal(pkg.attention_kv4(q, *args), want)
+    assert torch.equal(pkg.attention_kv4(q.detach(), *args), want)
