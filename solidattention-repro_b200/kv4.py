@@ -230,6 +230,9 @@ def attention_kv4(query: torch.Tensor, pool: torch.Tensor, block_table: torch.Te
     if block_table.shape[1] == 0:  # no request holds a block: a column without one stands for it
         block_table = block_table.new_full((n, 1), -1)
         table = block_table.data_ptr()
+    if selected is not None and budget == 0:  # lists without room: the block of the newest token alone
+        selected, selected_count = seq_lens.new_zeros(n, groups, 1), seq_lens.new_zeros(n, groups)
+        ids, counts, budget = selected.data_ptr(), selected_count.data_ptr(), 1
     ws_bytes = _workspace_bytes(n, new, qh, heads, d, dev)
     ws = pool.new_empty(ws_bytes or 16)
     _call(dev, "attention_kv4", lib.sa_attention_kv4, q, _TYPES[query.dtype], query.stride(0),

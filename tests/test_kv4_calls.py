@@ -58,3 +58,14 @@ def test_a_query_that_requires_grad_is_refused_in_grad_mode(pkg, cuda):
     with torch.inference_mode():
         assert torch.equal(pkg.attention_kv4(q, *args), want)
     assert torch.equal(pkg.attention_kv4(q.detach(), *args), want)
+
+
+@pytest.mark.gpu
+def test_lists_without_room_attend_the_newest_block(pkg, cuda):
+    rng = np.random.default_rng(2)
+    pool, table = _cache(rng, 2, [70, 20], 2, 64, cuda)
+    args = [_query(rng, (2, 4, 64), torch.bfloat16, cuda), torch.as_tensor(pool, device=cuda), _i32(table, cuda),
+            _i32([70, 20], cuda)]
+    zero, counts = torch.zeros(2, 2, 3, dtype=torch.int32, device=cuda), _i32([[5, 0], [0, -1]], cuda)
+    want = pkg.attention_kv4(*args, selected=zero, selected_count=torch.zeros_like(counts))
+    assert torch.equal(pkg.attention_kv4(*args, selected=zero[..., :0].contiguous(), selected_count=counts), want)
