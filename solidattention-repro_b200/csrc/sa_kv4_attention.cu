@@ -174,6 +174,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2^k, -126 <= k <= 127.
 __device__ __forceinline__ float power_of_2(int k) { return __int_as_float((k + 127) << 23); }
 
+// E for a group's largest step, given as FP16 bits: 2^E is above it. Steps stay as they are
+// while the largest is in [2^-8, 1).
+__device__ __forceinline__ int step_exponent(uint32_t largest) {
+  const int exponent = static_cast<int>(largest >> 10) - 14;
+  return exponent > -8 && exponent <= 0 ? 0 : exponent;
+}
+
 // k of a power of two 2^k held as FP16 bits in the low half (k up to 16, one above FP16's largest exponent).
 __device__ __forceinline__ int step_log2(uint32_t bits) { return static_cast<int>(bits >> 10 & 31u) - 15; }
 
@@ -748,9 +755,7 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
           largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
           const uint32_t bits = step_bits[gr] & 0xffffu;
           if (largest < bits) continue;  // the same in every lane
-          // steps stay as they are while the largest is in [2^-8, 1)
-          int exponent = static_cast<int>(largest >> 10) - 14;
-          if (exponent > -8 && exponent <= 0) exponent = 0;
+          const int exponent = step_exponent(largest);
           const float keep = bits == 0 ? 0.0f : power_of_2(step_log2(bits) - exponent);
           step_bits[gr] = static_cast<uint32_t>(exponent + 15) * 0x04000400u;
           const __half2 unit = __half2half2(__float2half_rn(power_of_2(-exponent)));
@@ -895,14 +900,16 @@ __global__ void __launch_bounds__(Ring<NG, NT>::kWarps * 32, 1)
     // apart, 16 requests with 4 drafts each took 171 us instead of 150.)
     auto parts_rows = [&](const uint8_t* entry, int from, int to) {
       bool parts = false;
-      if (lane >= from && lane < to) {
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          const auto* at = reinterpret_cast<const uint16_t*>(entry + kv4_value_scale_at(kDim, lane, gr));
-          parts |= at[0] >= (step_bits[gr] & 0xffffu) || (at[kDim / 2] & 0x7c00u) == 0x7c00u;
-        }
+      for (int gr = 0; gr < NG; ++gr) {
+        const auto* at = reinterpret_cast<const uint16_t*>(entry + kv4_value_scale_at(kDim, lane, gr));
+        const uint32_t step = at[0];
+        uint32_t bound = step_bits[gr] & 0xffffu;
+        if (bound == 0)  // none yet: the one that the tokens seen by all rows will set
+          bound = (step_exponent(__reduce_max_sync(0xffffffffu, lane < from && step < 0x7c00u ? step : 0u)) + 15) << 10;
+        parts |= step >= bound || (at[kDim / 2] & 0x7c00u) == 0x7c00u;
       }
-      return __any_sync(0xffffffffu, parts);
+      return __any_sync(0xffffffffu, parts && lane >= from && lane < to);
     };
 
     int stage = 0, seen = 0;  // seen: tokens of a masked block that its last turn's rows saw
