@@ -185,7 +185,8 @@ SA_API sa_status sa_pack_kv_fp16(uint16_t* packed, const float* key,
  *
  *   minimum m = largest FP16 value <= the group's smallest element,
  *   step    s = smallest FP16 value >= (largest element - m) / 15,
- *   code    c = (x - m) / s rounded to nearest, ties to even (0 if s = 0),
+ *   code    c = (x - m) / s rounded to nearest, ties to even (0 if s = 0;
+ *             x - m is an FP32 difference),
  *   the value held is s * c + m: within s / 2 of x.
  *
  * Finite elements are first clamped to +-65504; a NaN or infinite element

@@ -7,11 +7,12 @@
 // group of 64, so its minimum and maximum take two shuffles each. (Eight
 // elements of four tokens a thread spent 2.5 times the instructions: prompts of
 // 99,991 tokens, 5 heads of 64, packed and read back in 145 us, now 86 us.)
-// Measured on the device: a prefix of 32,768 tokens, 8 heads of 128, read back in
-// 35 us (4.9 TB/s, 0.74 of the copy rate); a chunk of 8,192 tokens packed and
-// read back in 22 us (4.0 TB/s). Unpacking is bound by the memory pipeline,
-// packing by instructions (17 an element, two thirds of them for rows and scales
-// rather than codes).
+// Measured on the device: 32,768 tokens, 8 heads of 128, packed in 40 us in BF16,
+// 38 in FP16 and 52 in FP32, read back in 35, 35 and 71 us, against floors of 26,
+// 26 and 47; a chunk of 8,192 tokens in FP16 packed and read back in 21.4 us.
+// Packing is bound by instructions (81 % of the issue slots, 17 an element, two
+// thirds of them for rows and scales rather than codes), unpacking by the latency
+// of its loads and nearly by instructions (72 % of the slots, 12 an element).
 //
 // Rounding. The step is the smallest FP16 number s with 15 s >= max - minimum
 // (the difference rounded up; 15 s is exact in FP32, so the comparison decides

@@ -21,20 +21,26 @@
 // tile; the weights become the second product's operand by an 8x8 transpose of
 // registers (movmatrix).
 //
-// Rounding. FP32 queries are split into two FP16 parts. Weights are rounded to
-// FP16 once where the output is BF16 (2^-11 against its 2^-8) and split into
-// two parts otherwise. There the value codes are also centred, c - 8 with
-// minimum + 8 step (in two FP16 parts): over a long context the output is a
-// small difference of large sums otherwise, and the matrix unit's truncating
-// sums lost 1e-4 of it at 4,128 tokens (9e-7 for plain FP32). FP32 queries
-// centre the key codes too, and add the products of their small parts apart.
-// Logits, maxima, sums and partial results are FP32. The value
-// steps of each group of 64 elements are scaled by a power of two 2^-E that
-// follows the group's largest finite one, so that weight * step stays inside
-// FP16. Groups are separate output elements: a huge or NaN step of one leaves
-// the others as they are. Inside a group, steps more than 2^-14 below the
-// largest one that a warp has seen lose bits (they are FP16 subnormals then,
-// off by 2^-25 of 2^E), an error of 2^-24 of the group's largest value.
+// Rounding. FP32 queries are split into two FP16 parts. Where the output is
+// BF16, weights are rounded to FP16, and again when the step is multiplied in
+// (2^-11 each against the output's own 2^-8): the error against float64 is
+// 1.73e-3 where FP32 weights leave 1.66e-3 (8,192 tokens; 1.67e-3 and 1.65e-3
+// over 997). Weights in two parts would close that at 136 us for the 115 of 64
+// requests of 8K, 166 with centred codes. Other outputs have them in two parts.
+// There the value codes are also centred, c - 8 with minimum + 8 step (in two
+// FP16 parts): over a long context the output is a small difference of large
+// sums otherwise, and the matrix unit's truncating sums lost 1e-4 of it at
+// 4,128 tokens (9e-7 for plain FP32). FP32 queries centre the key codes too,
+// and add the products of their small parts apart. Logits, maxima, sums and
+// partial results are FP32.
+//
+// The value steps of each group of 64 elements are scaled by a power of two
+// 2^-E that follows the group's largest finite one, so that weight * step
+// stays inside FP16. Groups are separate output elements: a huge or NaN step
+// of one leaves the others as they are. Inside a group, steps more than 2^-14
+// below the largest one that a warp has seen lose bits (they are FP16
+// subnormals then, off by 2^-25 of 2^E), an error of 2^-24 of the group's
+// largest value.
 //
 // Work split. All (list, KV head, row tile) units' entries form one flat list;
 // every CTA takes an equal contiguous range of it, whatever the lengths, and
@@ -44,11 +50,12 @@
 // the CTA first where its whole range lies in one unit, and merge_kernel joins
 // them in the order of the list.
 //
-// Measured (device time, both launches; 32 query heads of 128 over 8): 64
-// requests of 8,192 tokens in BF16 116 us, 5.2 TB/s of cache, 0.79 of the copy
-// rate; FP16 168 us and FP32 195 us, bound by instructions (weights and, for
-// FP32, queries in two parts). One request of 997 tokens: 10.8 us, launches,
-// the chain of dependent reads and code that runs once.
+// Measured (device time, both launches, bursts of ten calls; 32 query heads of
+// 128 over 8): 64 requests of 8,192 tokens in BF16 115 us, 5.3 TB/s of cache,
+// 0.80 of the copy rate (136 us, 0.68, in a loop of seconds, where the power
+// cap lowers the clock); FP16 164 us and FP32 193 us, bound by instructions
+// (weights and, for FP32, queries in two parts). One request of 997 tokens: 10.4
+// to 11 us, launches, the chain of dependent reads and code that runs once.
 #include <algorithm>
 #include <type_traits>
 
@@ -59,10 +66,13 @@ namespace {
 
 constexpr int kMaxLists = 8192;
 // Warps of an attention CTA, one CTA an SM: 16 of 128 registers, 12 of 168, or 8
-// of 255 for the larger tiles. (32 requests of 8K, 8 rows a tile: 66 us with 12 warps, 73
-// with 8, 74 with two CTAs of 8 warps at 128 registers, FP32 queries 105, 107 and
-// 143; 10 and 14 warps, which the four schedulers share unevenly, 75 and 74. 16
-// rows a tile: 147 us with 8 warps, 153 with 12.)
+// of 255 for the larger tiles. Medians over eight places of the cache in memory,
+// between which one binary differs by 1 to 8 %: 32 requests of 8K, 8 rows a tile,
+// 67.2 us with 12 warps (66.9 to 68.6, once 72.9), 73.6 with 8 (73.2 to 73.8), 64
+// requests 115 and 130; FP32 queries 105 and 108; head_dim 64 77.7 with 16 warps,
+// 81.3 with 12, 97 with 8. 16 rows a tile, 16 query heads a KV head: 63.6 us with
+// 8 warps, 71.6 with 12 (400 to 560 bytes of spills a thread); four drafts of
+// two sets of ragged requests 149 and 153, 182 and 175.
 __host__ __device__ constexpr int attention_warps(int head_dim, int tile) {
   return tile > 8 || head_dim > 128 ? 8 : head_dim == 64 ? 16 : 12;
 }
@@ -1118,7 +1128,7 @@ __device__ __forceinline__ void store1(void* base, int64_t i, int type, float x)
 // CTA a query row, its warps sharing the row's parts, of which few units can have
 // hundreds. Otherwise one CTA a unit and a warp a row: most of the cost is then
 // finding the parts, and many units have none left to join (512 requests of 100
-// tokens: 66 us with a CTA a row, 46 us so).
+// tokens: 62 us with a CTA a row, 47 us so).
 template <int NG, int WARPS, bool SHARED>
 __global__ void __launch_bounds__(WARPS * 32) merge_kernel(const Kv4AttnParams p, int tile) {
   constexpr int kDim = 64 * NG, kPerLane = kDim / 32;
@@ -1207,7 +1217,9 @@ sa_status launch(const Kv4AttnParams& p, int lists, cudaStream_t stream) {
   SA_CUDA_TRY(launch_kernel(kernel, dim3(p.ctas), dim3(Ring<NG, NT>::kWarps * 32), smem, stream, false, p));
   // A warp a row where units have some four parts (all warps' ranges over the
   // units), else a CTA a row: 16, 32 and 64 requests of 8K (14, 7 and 3.5 parts)
-  // took 44, 67 and 116 us with a CTA a row, 49, 68 and 114 us with a warp.
+  // took 43.1, 67.3 and 117.4 us with a CTA a row, 48.4, 69.0 and 115.2 us with a
+  // warp (medians over eight places of the cache; 0.5, 1.9 and 1.8 us between the
+  // ends of either).
   const int units = lists * p.units_per_list, rows = std::min(p.rows, 8 * NT);
   const auto merge = [&](auto kernel_, int grid, int warps) {
     return launch_kernel(kernel_, dim3(grid), dim3(warps * 32), 0, stream, false, p, 8 * NT);

@@ -156,7 +156,7 @@ def test_rows_see_their_own_tokens_with_every_element_bounded(pkg, cuda, dtype, 
         for k in range(min(new, length)):
             for head in range(2):
                 for g in range(2):
-                    _set_value(pool, table, 128, b, length - 1 - k, head, g, 2.0 ** (new - k - 3), 4.0 ** (new - k))
+                    _set_value(pool, table, 128, b, length - 1 - k, head, g, 2.0 ** (new - k - 3), 3.0 ** (new - k))
     _check_elements(pkg, _query(rng, (len(lens), new, 2 * group, 128), dtype, cuda), pool, table, lens, cuda)
 
 
