@@ -208,3 +208,27 @@ def test_attention_over_finite_rows_is_finite(pkg, cuda, query, out, tokens):
     # the sum of equal values: FP32 sums (2^-19) and one rounding; BF16 weights as above
     tol = np.abs(want) * (HALF_STEP[got.dtype] + 2.0 ** -19 + (2.0 ** -10 if got.dtype == torch.bfloat16 else 0)) + 0.1
     assert (np.abs(got.double().cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new, group, d", [(4, 4, 128), (9, 1, 64), (3, 2, 256)])
+def test_ordinary_later_values_and_large_later_keys(pkg, cuda, dtype, new, group, d):
+    """Other values in the newest tokens leave the rows before them byte by byte as they are; keys that are far larger
+    there may move their running maximum, so those rows are held to float64 again."""
+    rng = np.random.default_rng(d + new)
+    lens = [60 + new, 1000, new + 1, 31 + new]
+    pool, table = _cache(rng, 4, lens, 2, d, cuda)
+    q = _query(rng, (4, new, 2 * group, d), dtype, cuda)
+    clean = _check_elements(pkg, q, pool, table, lens, cuda)
+    _, _, _, key_step, _ = oracle4.positions(d)
+    for b, length in enumerate(lens):
+        for head in range(2):
+            for g in range(d // 64):
+                _set_value(pool, table, d, b, length - 1, head, g, 0.21, -1.3)
+    out = _check_elements(pkg, q, pool, table, lens, cuda)
+    assert torch.equal(out[:, :-1], clean[:, :-1]) and not torch.equal(out[:, -1], clean[:, -1])
+    for b, length in enumerate(lens):
+        for at in key_step[(length - 1) % BLOCK, ::GROUP] // 2:
+            pool.view(np.float16)[table[b, (length - 1) // BLOCK], :, at] = 9.0
+    _check_elements(pkg, q, pool, table, lens, cuda)
